@@ -163,6 +163,76 @@ int rpfq_gemm_plan_sm100(const RpfqGemmArgs* args, RpfqGemmPlan* plan);
 int rpfq_act_quant_sm100(const uint16_t* x, int64_t ldx, uint16_t* xq, int64_t ldq, int64_t m, int32_t k,
                          int32_t num_bits, rpfq_stream_t stream);
 
+/* Rows to int8 codes with one fp32 scale per row: the tokens of an activation
+ * matrix, or the output channels of a weight matrix [n, k]. x is [m, k] fp16
+ * (fp32 with x_f32 != 0), row stride ldx; q is [m, k] int8, row stride ldq.
+ *   t = max(amax |x|, 1e-30); q = rint(fl(x * fl(fl(1 / t) * 127))); scale = t / 127
+ * (half to even, fp32 steps). A row with a NaN or an infinity gets codes of
+ * zero and a scale of NaN. No counterpart in the reference, whose quantizers
+ * return to fp16 (ActivationQuantSTE.forward,
+ * RPFQ-ViT-main/quant_models/quant_i.py:442-455). */
+int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                             int64_t m, int32_t k, rpfq_stream_t stream);
+
+/* y[m, n] = act(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]) +
+ * residual[m, n] of int8 codes x [m, k] and w [n, k] with one scale per token
+ * and one per output channel: exact int32 sums on the tensor cores, scaled in
+ * fp32, fp16 or fp32 output. The 8-bit form of rpfq_gemm_sm100; y may alias
+ * residual. Requirements: x and w 16-byte aligned with row strides that are
+ * multiples of 16 (any k up to 131071 within such rows); y, residual, bias and
+ * the scales aligned to their values, any n and any row strides >= n; the
+ * residual has y's dtype. Nothing is kept between calls. */
+typedef struct RpfqGemmI8Args {
+    const int8_t* x;          /* int8 [m, k], row stride ldx                            */
+    int64_t ldx;
+    const float* x_scale;     /* fp32 [m]                                               */
+    const int8_t* w;          /* int8 [n, k], row stride ldw                            */
+    int64_t ldw;
+    const float* w_scale;     /* fp32 [n]                                               */
+    const void* bias;         /* fp16 [n] (fp32 with RPFQ_GEMM_BIAS_F32) or NULL        */
+    const void* residual;     /* [m, n] fp16 (fp32 with RPFQ_GEMM_RESIDUAL_F32) or NULL */
+    int64_t ldr;
+    void* y;                  /* [m, n] fp16 (fp32 with RPFQ_GEMM_OUT_F32), stride ldy  */
+    int64_t ldy;
+    int64_t m;
+    int32_t n, k;
+    int32_t activation;       /* RPFQ_ACT_NONE or RPFQ_ACT_GELU (erf)                   */
+    int32_t flags;            /* RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32 */
+} RpfqGemmI8Args;
+int rpfq_gemm_i8_sm100(const RpfqGemmI8Args* args, rpfq_stream_t stream);
+
+enum { RPFQ_POS_I32 = 0, RPFQ_POS_I64 = 1, RPFQ_POS_F32 = 2, RPFQ_POS_F64 = 3 }; /* types of a position */
+
+/* Rotary positions: pair j of the first 2 * pairs values of every head is
+ * turned by the angle position * inv_freq[j] and scaled by magnitude,
+ *   y_a = c (a cos - b sin), y_b = c (b cos + a sin),
+ * the pair lying at (j, j + pairs), or at (2j, 2j + 1) with interleaved != 0.
+ * The other values of a head are copied. transpose != 0 turns by the negative
+ * angle: the gradient of the plain call, given the gradient of its output. With
+ * axes == 2 the first half of the pairs uses positions[.., 0], the rest
+ * positions[.., 1]. Angles are formed and reduced in fp64. x and y are fp16
+ * (fp32 with f32 != 0) [batch, length, heads, dim] with strides in elements
+ * and unit stride inside a head; y may be x (same strides), which leaves the
+ * values past 2 * pairs untouched, and may not overlap x in any other way. */
+typedef struct RpfqRotaryArgs {
+    const void* x;
+    int64_t x_batch, x_token, x_head;   /* strides                                        */
+    void* y;
+    int64_t y_batch, y_token, y_head;
+    const void* positions;              /* [length, axes]; [batch, length, axes] when
+                                           position_batch = length * axes (0: shared)     */
+    int64_t position_batch;
+    const double* inv_freq;             /* [pairs]                                        */
+    int64_t batch, length;
+    int32_t heads, dim, pairs;
+    int32_t axes;                       /* 1 or 2                                         */
+    int32_t position_type;              /* RPFQ_POS_*                                     */
+    int32_t f32, interleaved, transpose;
+    float magnitude;
+    int32_t reserved;
+} RpfqRotaryArgs;
+int rpfq_rotary_sm100(const RpfqRotaryArgs* args, rpfq_stream_t stream);
+
 /* Patch unfold of the ViT / DeiT input: images [batch, channels, height,
  * width] (fp16, or fp32 with images_f32 != 0, contiguous) -> fp16 rows
  * patches[b * gh * gw + i * gw + j][c * patch^2 + y * patch + x] =

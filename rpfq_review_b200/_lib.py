@@ -25,6 +25,10 @@ ACT_GELU = 1
 GEMM_OUT_F32 = 1
 GEMM_RESIDUAL_F32 = 2
 GEMM_BIAS_F32 = 4
+POS_I32 = 0
+POS_I64 = 1
+POS_F32 = 2
+POS_F64 = 3
 ROUND_NEAREST_EVEN = 0
 ROUND_TIES_AWAY = 1
 
@@ -35,6 +39,9 @@ EXPORTED_SYMBOLS = (
     "rpfq_gemm_workspace_bytes",
     "rpfq_gemm_plan_sm100",
     "rpfq_act_quant_sm100",
+    "rpfq_quantize_rows_sm100",
+    "rpfq_gemm_i8_sm100",
+    "rpfq_rotary_sm100",
     "rpfq_patch_unfold_sm100",
     "rpfq_layernorm_sm100",
     "rpfq_layernorm_rows_sm100",
@@ -88,6 +95,34 @@ class RpfqGemmArgs(ctypes.Structure):
         ("flags", ctypes.c_int32), ("cta_pair", ctypes.c_int32),
         ("split_k", ctypes.c_int32), ("reserved", ctypes.c_int32),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class RpfqGemmI8Args(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p), ("ldr", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+        ("m", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+        ("activation", ctypes.c_int32), ("flags", ctypes.c_int32),
+    ]
+
+
+class RpfqRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_batch", ctypes.c_int64), ("x_token", ctypes.c_int64), ("x_head", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("y_batch", ctypes.c_int64), ("y_token", ctypes.c_int64), ("y_head", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("position_batch", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("batch", ctypes.c_int64), ("length", ctypes.c_int64),
+        ("heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("pairs", ctypes.c_int32),
+        ("axes", ctypes.c_int32), ("position_type", ctypes.c_int32),
+        ("f32", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("transpose", ctypes.c_int32),
+        ("magnitude", ctypes.c_float), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -148,6 +183,9 @@ def lib() -> ctypes.CDLL:
         L.rpfq_gemm_workspace_bytes.restype = ctypes.c_uint64
         L.rpfq_gemm_plan_sm100.argtypes = [ctypes.POINTER(RpfqGemmArgs), ctypes.POINTER(RpfqGemmPlan)]
         L.rpfq_act_quant_sm100.argtypes = [P, I64, P, I64, I64, I32, I32, P]
+        L.rpfq_quantize_rows_sm100.argtypes = [P, I32, I64, P, I64, P, I64, I32, P]
+        L.rpfq_gemm_i8_sm100.argtypes = [ctypes.POINTER(RpfqGemmI8Args), P]
+        L.rpfq_rotary_sm100.argtypes = [ctypes.POINTER(RpfqRotaryArgs), P]
         L.rpfq_patch_unfold_sm100.argtypes = [P, I32, I64, I32, I32, I32, I32, P, I64, P]
         L.rpfq_layernorm_sm100.argtypes = [P, I64, P, P, P, I64, I64, I32, ctypes.c_float, I32, P]
         L.rpfq_layernorm_rows_sm100.argtypes = [P, I64, I64, P, P, P, P, I64, I64, I32, ctypes.c_float, I32, P]
@@ -167,6 +205,7 @@ def lib() -> ctypes.CDLL:
         L.rpfq_last_error.restype = ctypes.c_char_p
         L.rpfq_device_error.argtypes = [ctypes.POINTER(I32)]
         for name in ("rpfq_prepack_sm100", "rpfq_gemm_sm100", "rpfq_gemm_plan_sm100", "rpfq_act_quant_sm100",
+                     "rpfq_quantize_rows_sm100", "rpfq_gemm_i8_sm100", "rpfq_rotary_sm100",
                      "rpfq_layernorm_sm100",
                      "rpfq_layernorm_rows_sm100", "rpfq_layernorm_ex_sm100",
                      "rpfq_wide_linear_sm100", "rpfq_wide_linear_noalloc_sm100", "rpfq_pack_linear_sm100",

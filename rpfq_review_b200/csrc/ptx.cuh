@@ -324,6 +324,28 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
         : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem]^T, int8 inputs, int32 accumulate (kind::i8,
+// K = 32 per instruction), for one CTA and for a CTA pair.
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive on the mbarrier at a shared::cluster address (this CTA or the peer)
 // when the pair MMAs issued so far by this thread have completed.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
@@ -409,6 +431,14 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_kmajor(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
     return (1u << 4)                                   // D format f32
            | (0u << 7) | (0u << 10)                    // A, B format f16
+           | (static_cast<uint32_t>(n >> 3) << 17)     // N >> 3
+           | (static_cast<uint32_t>(m >> 4) << 24);    // M >> 4
+}
+
+// Instruction descriptor for kind::i8: A = B = signed int8, D = int32, both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
+    return (2u << 4)                                   // D format s32
+           | (1u << 7) | (1u << 10)                    // A, B format s8
            | (static_cast<uint32_t>(n >> 3) << 17)     // N >> 3
            | (static_cast<uint32_t>(m >> 4) << 24);    // M >> 4
 }

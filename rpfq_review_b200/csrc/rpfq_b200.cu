@@ -24,8 +24,11 @@
 #include "decode_gemm.cuh"
 #include "embed.cuh"
 #include "gemm.cuh"
+#include "gemm_i8.cuh"
 #include "layernorm.cuh"
 #include "pack.cuh"
+#include "quantize_rows.cuh"
+#include "rotary.cuh"
 #include "vision_quant.cuh"
 #include "prepack.cuh"
 
@@ -168,6 +171,25 @@ int make_tmap_f16(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, 
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(RPFQ_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d) for a [%lld x %lld] matrix", (int)r,
+                    (long long)rows, (long long)cols);
+    return RPFQ_OK;
+}
+
+// Row-major int8 matrix [rows, cols], row stride ld bytes (a multiple of 16; any
+// cols), box [box_rows, 128 bytes], 128-B swizzle.
+int make_tmap_i8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    EncodeTiledFn fn;
+    int rc = encode_fn(&fn);
+    if (rc) return rc;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(RPFQ_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d) for an int8 [%lld x %lld] matrix", (int)r,
                     (long long)rows, (long long)cols);
     return RPFQ_OK;
 }
@@ -761,6 +783,112 @@ int gemm(const RpfqGemmArgs* a, cudaStream_t stream, RpfqGemmPlan* dry = nullptr
     return launch_gemm_bn<128, false>(a, st, stream, splits, false, false, dry);
 }
 
+// ---------------------------------------------------------------- int8 product
+constexpr int32_t kGemmI8MaxK = 131071;  // 128 * 128 * k < 2^31
+
+template <int BN, bool OUT_F32>
+int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t stream) {
+    using C = GemmI8TileCfg<BN>;
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t attr_status[kMaxDevices];
+    int dev = 0;
+    RPFQ_CUDA(cudaGetDevice(&dev));
+    std::call_once(once[dev], [dev]() {
+        attr_status[dev] = cudaFuncSetAttribute(gemm_i8_tile_kernel<BN, OUT_F32>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    });
+    RPFQ_CUDA(attr_status[dev]);
+    CUtensorMap tx, tw;
+    int rc = make_tmap_i8(&tx, a->x, a->m, a->k, a->ldx, p.x_rows);
+    if (!rc) rc = make_tmap_i8(&tw, a->w, a->n, a->k, a->ldw, BN);
+    if (rc) return rc;
+    const int64_t tiles = ((a->m + 127) / 128) * ((a->n + BN - 1) / BN);
+    if (tiles > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
+    RPFQ_CUDA(launch_kernel(gemm_i8_tile_kernel<BN, OUT_F32>, dim3(static_cast<unsigned>(tiles)), dim3(C::THREADS),
+                            C::SMEM_BYTES, stream, 1, tx, tw, p));
+    return RPFQ_OK;
+}
+
+// Vectors of four outputs: addresses and row strides of y and residual allow them.
+bool i8_vec_out(const RpfqGemmI8Args* a) {
+    const uintptr_t bytes = (a->flags & RPFQ_GEMM_OUT_F32) ? 16 : 8;
+    if (reinterpret_cast<uintptr_t>(a->y) % bytes || a->ldy % 4) return false;
+    return !a->residual || (reinterpret_cast<uintptr_t>(a->residual) % bytes == 0 && a->ldr % 4 == 0);
+}
+
+int gemm_i8(const RpfqGemmI8Args* a, cudaStream_t stream) {
+    const char* who = "rpfq_gemm_i8_sm100";
+    if (!a) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
+    if (a->m < 0 || a->n <= 0 || a->k <= 0)
+        return fail(RPFQ_ERR_INVALID, "%s: bad shape m=%lld n=%d k=%d", who, (long long)a->m, a->n, a->k);
+    if (a->k > kGemmI8MaxK)
+        return fail(RPFQ_ERR_UNSUPPORTED, "%s: k must be at most %d (int32 sums), got %d", who, kGemmI8MaxK, a->k);
+    if (a->m > (int64_t(1) << 31) - 256) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m too large", who);
+    if (a->flags & ~(RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32))
+        return fail(RPFQ_ERR_INVALID, "%s: unknown flags 0x%x", who, a->flags);
+    if (a->activation != RPFQ_ACT_NONE && a->activation != RPFQ_ACT_GELU)
+        return fail(RPFQ_ERR_INVALID, "%s: unknown activation %d", who, a->activation);
+    if (!a->w || !a->w_scale) return fail(RPFQ_ERR_INVALID, "%s: w and w_scale are required", who);
+    if (a->m == 0) return RPFQ_OK;
+    if (!a->x || !a->x_scale || !a->y) return fail(RPFQ_ERR_INVALID, "%s: x, x_scale and y are required", who);
+    if (a->ldx < a->k || a->ldx % 16 || a->ldw < a->k || a->ldw % 16)
+        return fail(RPFQ_ERR_INVALID, "%s: row strides of x and w must be >= k and multiples of 16", who);
+    if (!aligned16(a->x) || !aligned16(a->w)) return fail(RPFQ_ERR_INVALID, "%s: x and w must be 16-byte aligned", who);
+    if (a->ldy < a->n || (a->residual && a->ldr < a->n))
+        return fail(RPFQ_ERR_INVALID, "%s: row strides of y and residual must be >= n", who);
+    const uintptr_t esize = (a->flags & RPFQ_GEMM_OUT_F32) ? 4 : 2;
+    const uintptr_t bsize = (a->flags & RPFQ_GEMM_BIAS_F32) ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(a->y) % esize || reinterpret_cast<uintptr_t>(a->residual) % esize ||
+        reinterpret_cast<uintptr_t>(a->bias) % bsize || reinterpret_cast<uintptr_t>(a->x_scale) % 4 ||
+        reinterpret_cast<uintptr_t>(a->w_scale) % 4)
+        return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
+    if (a->residual && (((a->flags & RPFQ_GEMM_RESIDUAL_F32) != 0) != ((a->flags & RPFQ_GEMM_OUT_F32) != 0)))
+        return fail(RPFQ_ERR_UNSUPPORTED, "%s: the residual must have the output's dtype", who);
+    DeviceState* st;
+    int rc = device_state(&st);
+    if (rc) return rc;
+    GemmI8Params p;
+    p.x_scale = a->x_scale;
+    p.w_scale = a->w_scale;
+    p.bias = a->bias;
+    p.residual = a->residual;
+    p.ldr = a->ldr;
+    p.y = a->y;
+    p.ldy = a->ldy;
+    p.m = a->m;
+    p.n = a->n;
+    p.k = a->k;
+    p.activation = a->activation;
+    p.bias_f32 = (a->flags & RPFQ_GEMM_BIAS_F32) ? 1 : 0;
+    p.vec_out = i8_vec_out(a) ? 1 : 0;
+    p.x_rows = a->m >= 128 ? 128 : static_cast<int32_t>((a->m + 7) / 8 * 8);
+    p.err = st->err_word;
+    return (a->flags & RPFQ_GEMM_OUT_F32) ? launch_i8_tile<128, true>(a, p, stream)
+                                          : launch_i8_tile<128, false>(a, p, stream);
+}
+
+// ---------------------------------------------------------------- rotary positions
+template <typename T, bool INTERLEAVED>
+cudaError_t launch_rotary(int bytes, dim3 grid, cudaStream_t stream, const RotaryParams& p) {
+    if (bytes == 16) return launch_kernel(rotary_kernel<T, 16, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
+    if (bytes == 8) return launch_kernel(rotary_kernel<T, 8, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
+    return launch_kernel(rotary_kernel<T, 0, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
+}
+
+// Whether rows and runs of this call can move in vectors of `bytes`.
+bool rotary_vec(const RpfqRotaryArgs* a, int esize, int bytes, bool copy_rest) {
+    const int vec = bytes / esize;
+    const int run = a->interleaved ? 2 * a->pairs : a->pairs;
+    if (run % vec || (2 * a->pairs) % vec || (copy_rest && (a->dim - 2 * a->pairs) % vec)) return false;
+    if (reinterpret_cast<uintptr_t>(a->x) % bytes || reinterpret_cast<uintptr_t>(a->y) % bytes) return false;
+    // a stride of an axis of one entry is never used
+    const int64_t strides[6] = {a->batch > 1 ? a->x_batch : 0, a->length > 1 ? a->x_token : 0, a->heads > 1 ? a->x_head : 0,
+                                a->batch > 1 ? a->y_batch : 0, a->length > 1 ? a->y_token : 0, a->heads > 1 ? a->y_head : 0};
+    for (int64_t s : strides)
+        if (s % vec) return false;
+    return true;
+}
+
 // ---------------------------------------------------------------- packed-layer validation
 int check_layer(const RpfqPackedLinear* l, const char* who) {
     if (!l) return fail(RPFQ_ERR_INVALID, "%s: null layer", who);
@@ -907,6 +1035,98 @@ int rpfq_act_quant_sm100(const uint16_t* x, int64_t ldx, uint16_t* xq, int64_t l
     RPFQ_CUDA(launch_kernel(act_quant_kernel, dim3(static_cast<unsigned>(blocks)), dim3(warps * 32), 0,
                             static_cast<cudaStream_t>(stream), 1, p));
     RPFQ_CUDA(cudaGetLastError());
+    return RPFQ_OK;
+}
+
+int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                             int64_t m, int32_t k, rpfq_stream_t stream) {
+    const char* who = "rpfq_quantize_rows_sm100";
+    if (m < 0 || k <= 0) return fail(RPFQ_ERR_INVALID, "%s: bad shape m=%lld k=%d", who, (long long)m, k);
+    if (m == 0) return RPFQ_OK;
+    if (!x || !q || !scale) return fail(RPFQ_ERR_INVALID, "%s: null pointer", who);
+    if (ldx < k || ldq < k) return fail(RPFQ_ERR_INVALID, "%s: row strides must be >= k", who);
+    if (reinterpret_cast<uintptr_t>(x) % (x_f32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4)
+        return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
+    DeviceState* st;
+    int rc = device_state(&st);
+    if (rc) return rc;
+    QuantizeRowsParams p;
+    p.x = x;
+    p.ldx = ldx;
+    p.q = q;
+    p.ldq = ldq;
+    p.scale = scale;
+    p.m = m;
+    p.k = k;
+    const int64_t blocks = (m + 7) / 8;
+    if (blocks > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m too large", who);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    RPFQ_CUDA(x_f32 ? launch_kernel(quantize_rows_kernel<float>, grid, dim3(256), 0, cs, 1, p)
+                    : launch_kernel(quantize_rows_kernel<__half>, grid, dim3(256), 0, cs, 1, p));
+    return RPFQ_OK;
+}
+
+int rpfq_gemm_i8_sm100(const RpfqGemmI8Args* args, rpfq_stream_t stream) {
+    return gemm_i8(args, static_cast<cudaStream_t>(stream));
+}
+
+int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
+    const char* who = "rpfq_rotary_sm100";
+    if (!a) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
+    if (a->batch < 0 || a->length < 0 || a->heads < 0 || a->dim <= 0)
+        return fail(RPFQ_ERR_INVALID, "%s: bad shape", who);
+    if (a->pairs <= 0 || a->pairs > a->dim / 2)
+        return fail(RPFQ_ERR_INVALID, "%s: 2 * pairs must be in 2..dim (pairs=%d dim=%d)", who, a->pairs, a->dim);
+    if (a->pairs > kRotaryTable) return fail(RPFQ_ERR_UNSUPPORTED, "%s: at most %d pairs", who, kRotaryTable);
+    if ((a->axes != 1 && a->axes != 2) || a->pairs % a->axes)
+        return fail(RPFQ_ERR_INVALID, "%s: axes must be 1 or 2 and divide pairs (axes=%d pairs=%d)", who, a->axes, a->pairs);
+    if (a->position_type < RPFQ_POS_I32 || a->position_type > RPFQ_POS_F64)
+        return fail(RPFQ_ERR_INVALID, "%s: unknown position type %d", who, a->position_type);
+    if (a->batch == 0 || a->length == 0 || a->heads == 0) return RPFQ_OK;
+    if (!a->x || !a->y || !a->positions || !a->inv_freq) return fail(RPFQ_ERR_INVALID, "%s: null pointer", who);
+    if (a->heads > 65535) return fail(RPFQ_ERR_UNSUPPORTED, "%s: at most 65535 heads", who);
+    const int esize = a->f32 ? 4 : 2;
+    const int psize = (a->position_type == RPFQ_POS_I32 || a->position_type == RPFQ_POS_F32) ? 4 : 8;
+    if (reinterpret_cast<uintptr_t>(a->x) % esize || reinterpret_cast<uintptr_t>(a->y) % esize ||
+        reinterpret_cast<uintptr_t>(a->positions) % psize || reinterpret_cast<uintptr_t>(a->inv_freq) % 8)
+        return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
+    if (a->x == a->y && ((a->batch > 1 && a->x_batch != a->y_batch) || (a->length > 1 && a->x_token != a->y_token) ||
+                         (a->heads > 1 && a->x_head != a->y_head)))
+        return fail(RPFQ_ERR_INVALID, "%s: in place, x and y must have the same strides", who);
+    DeviceState* st;
+    int rc = device_state(&st);
+    if (rc) return rc;
+    const bool copy_rest = a->x != a->y;
+    RotaryParams p;
+    p.x = a->x;
+    p.y = a->y;
+    p.xb = a->x_batch, p.xl = a->x_token, p.xh = a->x_head;
+    p.yb = a->y_batch, p.yl = a->y_token, p.yh = a->y_head;
+    p.positions = a->positions;
+    p.pos_b = a->position_batch;
+    p.inv_freq = a->inv_freq;
+    p.tokens = a->batch * a->length;
+    p.length = static_cast<int32_t>(a->length);
+    p.heads = a->heads;
+    p.dim = a->dim;
+    p.pairs = a->pairs;
+    p.axes = a->axes;
+    p.pos_type = a->position_type;
+    p.copy_rest = copy_rest ? 1 : 0;
+    p.magnitude = a->magnitude;
+    p.sign = a->transpose ? -1.0f : 1.0f;
+    p.token_tile = std::max(1, std::min(32, kRotaryTable / a->pairs));
+    p.head_tile = a->heads;
+    const int64_t blocks = (p.tokens + p.token_tile - 1) / p.token_tile;
+    if (blocks > 0x7fffffff || a->length > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: too many tokens", who);
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((p.heads + p.head_tile - 1) / p.head_tile));
+    const int bytes = rotary_vec(a, esize, 16, copy_rest) ? 16 : (rotary_vec(a, esize, 8, copy_rest) ? 8 : 0);
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    RPFQ_CUDA((a->f32 ? (a->interleaved ? launch_rotary<float, true>(bytes, grid, cs, p)
+                                        : launch_rotary<float, false>(bytes, grid, cs, p))
+                      : (a->interleaved ? launch_rotary<__half, true>(bytes, grid, cs, p)
+                                        : launch_rotary<__half, false>(bytes, grid, cs, p))));
     return RPFQ_OK;
 }
 

@@ -44,12 +44,26 @@ class PackedPhaseLinear(nn.Module):
     buffer. With ``cache_dense=False`` only the packed planes stay resident:
     calls of at most ``ops.FUSED_DECODE_MAX_ROWS`` rows decode the codes inside
     the GEMM, larger calls decode into a temporary dense matrix first.
+
+    ``compute="int8"`` runs the product in 8-bit integers: the decoded
+    coefficients are quantized once to int8 with a scale per output channel
+    (half the memory of the fp16 matrix), every call quantizes its activations
+    to 8 bits with a scale per token (``ops.linear_int8``). It takes the place of
+    the activation quantizers above and needs ``cache_dense=True``.
     """
 
     def __init__(self, in_features: int, out_features: int, stages: int = 2, code_bits: int = 2,
                  enable_act_quant: bool = False, act_num_bits: int = 4, activation: str = "none",
-                 rounding: str = "rne", cache_dense: bool = True, vision_quant: dict | None = None, device=None):
+                 rounding: str = "rne", cache_dense: bool = True, vision_quant: dict | None = None, device=None,
+                 compute: str = "fp16"):
         super().__init__()
+        if compute not in ("fp16", "int8"):
+            raise ValueError(f"compute must be 'fp16' or 'int8', got {compute!r}")
+        if compute == "int8" and enable_act_quant:
+            raise ValueError("compute='int8' quantizes the activations itself: use enable_act_quant=False")
+        if compute == "int8" and not cache_dense:
+            raise ValueError("compute='int8' keeps the 8-bit coefficients: use cache_dense=True")
+        self.compute = compute
         if in_features % 2 or out_features % 2:
             raise ValueError("Complex-phase QAT requires even in/out features.")
         self.in_features, self.out_features = in_features, out_features
@@ -69,6 +83,9 @@ class PackedPhaseLinear(nn.Module):
                 self.add_module(f"{tag}_s{s}", PhasePlane(n_cp, k_cp, code_bits, device))
         self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float16, device=device))
         self.register_buffer("dense", None, persistent=False)
+        # compute="int8": the coefficients as int8 codes [N, K] and fp32 scales [N]
+        self.register_buffer("codes8", None, persistent=False)
+        self.register_buffer("scale8", None, persistent=False)
         self._bias32 = None  # (version, fp32 copy of bias) for the epilogue
 
     # -- construction ---------------------------------------------------------
@@ -133,7 +150,12 @@ class PackedPhaseLinear(nn.Module):
 
     def prepack(self) -> torch.Tensor:
         """Decode the packed planes once (K1). Layers whose real dims are not
-        multiples of 8 keep a zero-padded copy ``[N8, K8]`` for the GEMM."""
+        multiples of 8 keep a zero-padded copy ``[N8, K8]`` for the GEMM. With
+        ``compute="int8"`` the decoded rows are quantized and only their codes
+        and scales are kept; returns the codes."""
+        if self.compute == "int8":
+            self.codes8, self.scale8 = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
+            return self.codes8
         self.dense = self._decode_dense()
         return self.dense
 
@@ -150,6 +172,12 @@ class PackedPhaseLinear(nn.Module):
         if out_dtype is None:
             out_dtype = out.dtype if out is not None else (x.dtype if x.dtype in (torch.float16, torch.float32)
                                                            else torch.float16)
+        if self.compute == "int8":
+            if self.codes8 is None or self.codes8.device != x.device:
+                self.prepack()
+            xf = x if x.dtype in (torch.float16, torch.float32) else x.to(torch.float16)
+            return ops.linear_int8(xf, self.codes8, self.scale8, self._bias_f32(), residual, self.activation, out,
+                                   out_dtype)
         x16 = x if x.dtype == torch.float16 else x.to(torch.float16)
         act_bits = 0 if prequantized else self.act_bits
         if self.vision_quant is not None and not prequantized:
@@ -199,6 +227,7 @@ class PackedPhaseLinear(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, stages={self.stages}, "
                 f"code_bits={self.code_bits}, act_bits={self.act_bits}, activation={self.activation}"
+                + (", compute=int8" if self.compute == "int8" else "")
                 + (f", vision_quant={self.vision_quant}" if self.vision_quant else ""))
 
 

@@ -501,6 +501,296 @@ def act_quant(x: torch.Tensor, num_bits: int, out: torch.Tensor | None = None) -
     return out.reshape(x.shape)
 
 
+# ---------------------------------------------------------------------------
+# 8-bit linear path
+# ---------------------------------------------------------------------------
+
+GEMM_INT8_MAX_K = 131071  # 128 * 128 * k < 2^31: the int32 sums cannot overflow
+
+
+def _forward_only(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
+
+
+def _same_device(name: str, device: torch.device, **tensors) -> None:
+    for what, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: {what} is on {t.device}, not on {device}")
+
+
+def _float_type(t: torch.Tensor, name: str) -> bool:
+    """True for float32, False for float16; anything else is refused."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"{name} must be float16 or float32, got {t.dtype}")
+    return t.dtype == torch.float32
+
+
+def _code_rows(q: torch.Tensor, k: int, name: str):
+    """``q[..., k]`` int8 as 2-D rows that start on 16 bytes (what the TMA loads
+    need): rows of another stride or address are copied into such rows."""
+    q2, ld = _rows(q, k, name)
+    rows = q2.shape[0]
+    if rows <= 1:
+        ld = (k + 15) // 16 * 16
+    if ld < k or ld % 16 or q2.data_ptr() % 16:
+        ld = (k + 15) // 16 * 16
+        buf = torch.empty((rows, ld), dtype=torch.int8, device=q.device)
+        buf[:, :k] = q2
+        q2 = buf
+    return q2, ld
+
+
+def _quantize_rows(x: torch.Tensor, k: int, f32: bool):
+    """Codes [m, ld] (k columns used, rows on 16 bytes) and scales [m] of ``x[..., k]``."""
+    x2, ldx = _rows(x, k, "x")
+    if ldx < k:  # rows that overlap (expanded): one copy
+        x2, ldx = x2.contiguous(), k
+    m, ld = x2.shape[0], (k + 15) // 16 * 16
+    q = torch.empty((m, ld), dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _lib.check(_lib.lib().rpfq_quantize_rows_sm100(x2.data_ptr(), int(f32), ldx, q.data_ptr(), ld, scale.data_ptr(),
+                                                   m, k, _stream(x.device)), "rpfq_quantize_rows_sm100")
+    if m:
+        _count_launch()
+    return q, scale, ld
+
+
+def quantize_rows(x: torch.Tensor):
+    """8-bit codes and one scale per row of fp16 or fp32 ``x[..., k]``
+    (``rpfq_quantize_rows_sm100``): ``t = max(amax |x|, 1e-30)``,
+    ``codes = rint(x * (1 / t * 127))`` in fp32 steps, ``scale = t / 127``.
+    Returns int8 ``[..., k]`` (rows padded to a multiple of 16 bytes in memory,
+    so a view when k is none) and fp32 ``[...]``. A row that holds a NaN or an
+    infinity gets codes of zero and a scale of NaN. The tokens of an activation
+    matrix, or the output channels of a weight ``[n, k]``."""
+    f32 = _float_type(x, "x")
+    _forward_only("quantize_rows", x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(x.shape)}")
+    k = x.shape[-1]
+    with torch.cuda.device(x.device):
+        q, scale, ld = _quantize_rows(x, k, f32)
+    if ld == k:
+        return q.view(x.shape), scale.view(x.shape[:-1])
+    codes = q.view(*x.shape[:-1], ld)[..., :k]
+    return codes, scale.view(x.shape[:-1])
+
+
+def _product_int8(name: str, lead, x_ptr: int, ldx: int, x_scale: torch.Tensor, m: int, w: torch.Tensor,
+                  w_scale: torch.Tensor, bias, residual, activation, out, out_dtype) -> torch.Tensor:
+    """The checks and the launch that gemm_int8 and linear_int8 share."""
+    n, k = w.shape
+    device = x_scale.device
+    _require(w_scale, "w_scale", torch.float32)
+    if w_scale.numel() != n:
+        raise ValueError(f"{name}: w_scale must hold {n} values, got {w_scale.numel()}")
+    w2, ldw = _code_rows(w, k, "w")
+    w_scale = w_scale.contiguous()
+    if activation not in _ACT:
+        raise ValueError(f"{name}: unknown activation {activation!r}")
+    if bias is not None:
+        if not bias.is_cuda or bias.numel() != n:
+            raise ValueError(f"{name}: bias must be a CUDA tensor of {n} values")
+        bias = bias.contiguous()
+    if out is None:
+        out = torch.empty((*lead, n), dtype=out_dtype, device=device)
+    y2, ldy = _rows(out, n, "out")
+    if y2.data_ptr() != out.data_ptr() or y2.shape[0] != m or (m > 1 and ldy < n):
+        raise ValueError(f"{name}: out must be a row-major view of {m} rows with unit column stride")
+    r2, ldr = (None, 0)
+    if residual is not None:
+        if not residual.is_cuda:
+            raise ValueError("residual must be a CUDA tensor")
+        r2, ldr = _rows(residual, n, "residual")
+        if r2.shape[0] != m:
+            raise ValueError(f"{name}: residual rows do not match x")
+        if ldr < n:
+            r2, ldr = r2.contiguous(), n
+    _same_device(name, device, w=w, w_scale=w_scale, bias=bias, residual=residual, out=out)
+    a = _lib.RpfqGemmI8Args(x=x_ptr, ldx=ldx, x_scale=x_scale.data_ptr(), w=w2.data_ptr(), ldw=ldw,
+                            w_scale=w_scale.data_ptr(), bias=_p(bias), residual=_p(r2), ldr=ldr, y=y2.data_ptr(),
+                            ldy=ldy, m=m, n=n, k=k, activation=_ACT[activation], flags=_flags(out, r2, bias))
+    _lib.check(_lib.lib().rpfq_gemm_i8_sm100(ctypes.byref(a), _stream(device)), "rpfq_gemm_i8_sm100")
+    if m:
+        _count_launch()
+    return out
+
+
+def _check_codes(name: str, w: torch.Tensor) -> None:
+    _require(w, "w", torch.int8)
+    if w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0:
+        raise ValueError(f"{name}: w must be [n, k] with n, k > 0, got {tuple(w.shape)}")
+
+
+def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+              bias: torch.Tensor | None = None, residual: torch.Tensor | None = None, activation="none",
+              out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """``act(x_scale[..., None] * w_scale * (x @ w.T) + bias) + residual`` of
+    int8 codes ``x[..., k]`` and ``w[n, k]`` with a scale per token and per output
+    channel (``rpfq_gemm_i8_sm100``): exact int32 sums on the tensor cores
+    (k up to ``GEMM_INT8_MAX_K``), scaled in fp32. ``bias`` fp16 or fp32;
+    ``residual`` and ``out`` fp16 or fp32 alike (and may be the same tensor for
+    an in-place residual add). Code rows that do not start on 16 bytes are
+    copied into rows that do; :func:`quantize_rows` returns such rows."""
+    name = "gemm_int8"
+    _require(x, "x", torch.int8)
+    _check_codes(name, w)
+    _require(x_scale, "x_scale", torch.float32)
+    _forward_only(name, x_scale, w_scale, residual)
+    _same_device(name, x.device, x_scale=x_scale)
+    with torch.cuda.device(x.device):
+        x2, ldx = _code_rows(x, w.shape[1], "x")
+        m = x2.shape[0]
+        if x_scale.numel() != m:
+            raise ValueError(f"{name}: x_scale must hold one value per row ({m}), got {x_scale.numel()}")
+        return _product_int8(name, x.shape[:-1], x2.data_ptr(), ldx, x_scale.contiguous(), m, w, w_scale, bias,
+                             residual, activation, out, out_dtype)
+
+
+def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                residual: torch.Tensor | None = None, activation="none", out: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The 8-bit linear layer of fp16 or fp32 activations ``x[..., k]``: the rows
+    of x go through :func:`quantize_rows`, the codes through :func:`gemm_int8`
+    with the weight's codes and scales (``w, w_scale = quantize_rows(weight)``).
+    The other arguments as there."""
+    name = "linear_int8"
+    f32 = _float_type(x, "x")
+    _check_codes(name, w)
+    _forward_only(name, x, w_scale, residual)
+    with torch.cuda.device(x.device):
+        q, scale, ld = _quantize_rows(x, w.shape[1], f32)
+        return _product_int8(name, x.shape[:-1], q.data_ptr(), ld, scale, q.shape[0], w, w_scale, bias, residual,
+                             activation, out, out_dtype)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+_POSITION = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32,
+             torch.float64: _lib.POS_F64}
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, axes: int = 1, scaling: str = "none",
+                       factor: float = 1.0, original_length: int | None = None, low: float = 1.0, high: float = 32.0,
+                       device=None):
+    """The ``(inv_freq, magnitude)`` that :func:`rotary` takes for ``rot_dim``
+    rotated values per head: fp64 ``[rot_dim / 2]``, ``base ** (-j / p)`` for the
+    p = rot_dim / 2 / axes pairs of each axis.
+
+    ``scaling`` stretches them for sequences ``factor`` times longer than the
+    model has seen:
+
+    * ``"linear"``: every frequency divided by ``factor`` (positions interpolated);
+    * ``"base"``: base times ``factor ** (d / (d - 2))``, d = rot_dim / axes: the
+      fastest pair keeps its frequency, the slowest is divided by ``factor``;
+    * ``"parts"``: by how often a pair turns within ``original_length``: at
+      least ``high`` turns keep the frequency, at most ``low`` divide it by
+      ``factor``, linear in between; magnitude ``0.1 ln(factor) + 1``.
+
+    The magnitude is 1 otherwise."""
+    if axes not in (1, 2):
+        raise ValueError(f"rotary_frequencies: axes must be 1 or 2, got {axes}")
+    if rot_dim <= 0 or rot_dim % (2 * axes):
+        raise ValueError(f"rotary_frequencies: rot_dim must be a positive multiple of {2 * axes}, got {rot_dim}")
+    if not base > 0 or not factor >= 1:
+        raise ValueError(f"rotary_frequencies: base must be positive and factor at least 1, got {base}, {factor}")
+    per = rot_dim // 2 // axes
+    magnitude = 1.0
+    if scaling == "base":
+        if per < 2:
+            raise ValueError("rotary_frequencies: scaling 'base' needs at least two pairs per axis")
+        base = base * factor ** (per / (per - 1))
+    elif scaling not in ("none", "linear", "parts"):
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    freq = base ** (-torch.arange(per, dtype=torch.float64) / per)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "parts":
+        if not original_length or not high > low:
+            raise ValueError("rotary_frequencies: scaling 'parts' needs original_length and high > low")
+        turns = original_length * freq / (2.0 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        freq = freq * (keep + (1.0 - keep) / factor)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return freq.repeat(axes).to(device), magnitude
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, layout: str = "half", axes: int = 1,
+           magnitude: float = 1.0, transpose: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions on fp16 or fp32 heads ``x[L, H, D]`` or ``[B, L, H, D]``
+    (any strides, unit stride inside a head), ``rpfq_rotary_sm100``: pair j of
+    the first ``2 * inv_freq.numel()`` values of each head turns by
+    ``positions * inv_freq[j]`` (fp64 angles) and is scaled by ``magnitude``; the
+    other values are copied.
+
+    ``layout``: pairs at ``(j, j + P)`` (``"half"``) or ``(2j, 2j + 1)``
+    (``"interleaved"``). ``positions``: int32, int64, fp32 or fp64, ``[L]`` or
+    ``[B, L]``; with ``axes=2`` a trailing dimension of two, of which the first half
+    of the pairs takes the first (a patch's row) and the rest the second (its
+    column). ``out`` may be ``x`` (in place), e.g. the query and key heads of a
+    qkv product's rows: ``q = qkv.view(B, L, 3 * H, D)[:, :, :2 * H]``. It must
+    not overlap x in any other way.
+
+    No autograd: ``transpose=True`` turns the other way, which maps the gradient
+    of the output to the gradient of x."""
+    name = "rotary"
+    f32 = _float_type(x, "x")
+    _forward_only(name, x)
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{name}: x must be [L, H, D] or [B, L, H, D], got {tuple(x.shape)}")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"{name}: layout must be 'half' or 'interleaved', got {layout!r}")
+    if axes not in (1, 2):
+        raise ValueError(f"{name}: axes must be 1 or 2, got {axes}")
+    _require(inv_freq, "inv_freq", torch.float64)
+    L, H, D = x.shape[-3:]
+    B = x.shape[0] if x.dim() == 4 else 1
+    pairs = inv_freq.numel()
+    if pairs == 0 or 2 * pairs > D or pairs % axes:
+        raise ValueError(f"{name}: inv_freq must hold 1..{D // 2} values, a multiple of axes, got {pairs}")
+    if not positions.is_cuda or positions.dtype not in _POSITION:
+        raise ValueError(f"{name}: positions must be an int32, int64, float32 or float64 CUDA tensor")
+    tail = (axes,) if axes > 1 else ()
+    shape = tuple(positions.shape)
+    if shape == (L, *tail):
+        per_sequence = 0
+    elif x.dim() == 4 and shape == (B, L, *tail):
+        per_sequence = L * axes
+    else:
+        raise ValueError(f"{name}: positions must be {(L, *tail)} or {(B, L, *tail)}, got {shape}")
+    if x.stride(-1) != 1 and D > 1:
+        if out is x:
+            raise ValueError(f"{name}: in place, a head must have unit stride")
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"{name}: out must be {tuple(x.shape)} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
+    elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or (D > 1 and out.stride(-1) != 1):
+        raise ValueError(f"{name}: out must not be expanded and must have unit stride inside a head")
+    _same_device(name, x.device, positions=positions, inv_freq=inv_freq, out=out)
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    xs, ys = x.stride(), out.stride()
+    a = _lib.RpfqRotaryArgs(x=x.data_ptr(), x_batch=xs[0] if x.dim() == 4 else 0, x_token=xs[-3], x_head=xs[-2],
+                            y=out.data_ptr(), y_batch=ys[0] if x.dim() == 4 else 0, y_token=ys[-3], y_head=ys[-2],
+                            positions=positions.data_ptr(), position_batch=per_sequence,
+                            inv_freq=inv_freq.data_ptr(), batch=B, length=L, heads=H, dim=D, pairs=pairs, axes=axes,
+                            position_type=_POSITION[positions.dtype], f32=int(f32),
+                            interleaved=int(layout == "interleaved"), transpose=int(bool(transpose)),
+                            magnitude=float(magnitude))
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().rpfq_rotary_sm100(ctypes.byref(a), _stream(x.device)), "rpfq_rotary_sm100")
+    if x.numel():
+        _count_launch()
+    return out
+
+
+
 def wide_linear(x: torch.Tensor, layer: PackedLayer, dense: torch.Tensor | None, act_bits: int = 0,
                 activation="none", residual: torch.Tensor | None = None,
                 out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16,

@@ -17,6 +17,8 @@ fused into its epilogue; the patch embedding (a dense conv in the reference)
 runs through the same GEMM on unfolded patches. LayerNorm (+ activation
 quantization) is one kernel per row block; attention is PyTorch SDPA (cuDNN)
 or, with ``attention="rpfq"``, the library's tcgen05 short-sequence kernel.
+``compute="int8"`` runs the packed linears in 8-bit integers; ``rotary`` turns
+the query and key heads by their place on the patch grid before attention.
 """
 
 from __future__ import annotations
@@ -72,6 +74,15 @@ def _trunc_normal(shape, std, gen):
     return torch.nn.init.trunc_normal_(torch.empty(shape), std=std, a=-2 * std, b=2 * std, generator=gen)
 
 
+def grid_positions(cfg: ViTConfig) -> torch.Tensor:
+    """int32 ``[tokens, 2]``: row and column of each token's patch, class
+    (+ distillation) tokens at the origin."""
+    side = cfg.img // cfg.patch
+    at = torch.arange(side * side, dtype=torch.int32)
+    grid = torch.stack([at // side, at % side], -1)
+    return torch.cat([torch.zeros((cfg.tokens - side * side, 2), dtype=torch.int32), grid])
+
+
 class PackedViT(nn.Module):
     """Inference ViT / DeiT with packed complex-phase linears.
 
@@ -83,13 +94,24 @@ class PackedViT(nn.Module):
     divided by ``sqrt(K)`` so activations stay in fp16 range (needed for the
     3/4-bit sweep, which the exporter cannot produce).
     Each layer's seed derives from its name and ``seed``.
+
+    ``compute="int8"``: every packed linear as 8-bit integers
+    (``PackedPhaseLinear(compute="int8")``; ``act_bits`` and ``vision_quant`` off).
+    ``rotary``: a dict of :func:`ops.rotary_frequencies` arguments (``base``, ...)
+    and optionally ``rot_dim`` (default: the head dim) and ``layout``; query and
+    key heads are then turned in place in the qkv rows, by the row of a token's
+    patch in the first half of their pairs and by its column in the second; class
+    tokens stay at the origin.
     """
 
     def __init__(self, cfg: ViTConfig, device, seed: int = 0, act_bits: int = 0, weights: str = "random_init",
                  code_bits: int = 2, prepack: bool = True, vision_quant: dict | None = None,
-                 attention: str = "sdpa"):
+                 attention: str = "sdpa", compute: str = "fp16", rotary: dict | None = None):
         super().__init__()
         self.cfg = cfg
+        if compute == "int8" and (act_bits or vision_quant is not None):
+            raise ValueError("compute='int8' quantizes the activations itself: use act_bits=0 and no vision_quant")
+        self.compute = compute
         if attention not in ("sdpa", "rpfq"):
             raise ValueError(f"attention must be 'sdpa' or 'rpfq', got {attention!r}")
         # "rpfq": the library's tcgen05 short-sequence attention kernel (head
@@ -111,6 +133,14 @@ class PackedViT(nn.Module):
         ntok = 2 if cfg.distilled else 1
         self.register_buffer("cls_tokens", _trunc_normal((1, ntok, d), 0.02, g).half().to(dev))
         self.register_buffer("pos_embed", _trunc_normal((1, cfg.tokens, d), 0.02, g).half().to(dev))
+        self.rotary = None
+        if rotary is not None:
+            opts = dict(rotary)
+            layout, rot_dim = opts.pop("layout", "half"), opts.pop("rot_dim", d // cfg.heads)
+            inv_freq, magnitude = ops.rotary_frequencies(rot_dim, axes=2, device=dev, **opts)
+            self.rotary = dict(layout=layout, axes=2, magnitude=magnitude)
+            self.register_buffer("rotary_inv_freq", inv_freq, persistent=False)
+            self.register_buffer("rotary_positions", grid_positions(cfg).to(dev), persistent=False)
 
         def make(name, n_out, n_in, activation="none"):
             if weights == "random_init":
@@ -129,7 +159,7 @@ class PackedViT(nn.Module):
                 raise ValueError(f"unknown weights mode {weights!r}")
             return PackedPhaseLinear.from_packed(layer, enable_act_quant=act_bits > 0 or vision_quant is not None,
                                                  act_num_bits=act_bits or 4, activation=activation,
-                                                 vision_quant=vision_quant)
+                                                 vision_quant=vision_quant, compute=compute)
 
         self.blocks = nn.ModuleList()
         for i in range(cfg.depth):
@@ -238,6 +268,9 @@ class PackedViT(nn.Module):
             else:
                 h = ops.layernorm(x, blk.norm1_w, blk.norm1_b, cfg.eps, ab)
             qkv = blk.qkv(h, prequantized=pre)
+            if self.rotary is not None:  # query and key heads, in place
+                qk = qkv.view(B, L, 3 * H, hd)[:, :, :2 * H]
+                ops.rotary(qk, self.rotary_positions, self.rotary_inv_freq, out=qk, **self.rotary)
             if self.attention == "rpfq" and hd == 64 and L <= ops.ATTENTION_MAX_TOKENS:
                 a = ops.attention(qkv.view(B, L, 3 * d), H)
             else:

@@ -33,6 +33,10 @@ struct GemmI8Params {
     int32_t bias_f32;
     int32_t vec_out;         // y (and residual) rows take vectors of four values
     int32_t x_rows;          // rows of the x box: 128, or fewer when m is small
+    int32_t tma_out;         // pair kernel: y rows can be stored by TMA
+    int32_t tma_res;         // pair kernel: residual rows can be loaded by TMA
+    int32_t tail_tiles;      // pair kernel: last-wave tiles cut into `pieces` column pieces
+    int32_t pieces;          // 0: none; else 2 or 4
     int* err;
 };
 

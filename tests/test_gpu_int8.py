@@ -138,6 +138,40 @@ def test_gemm_int8_matches_fp64(cuda, m, n, k, out_dtype):
         _check(y, _product_ref(xq, xs, wq, ws, b, act, r, out_dtype))
 
 
+# enough 256 x 256 tiles for CTA pairs on 148 SMs: whole waves, last waves cut into two
+# and four column pieces, ragged rows and columns, one k-block and several
+MANY_ROWS = [(9500, 512, 200), (4900, 1000, 144), (6600, 1001, 96), (18900, 250, 33), (9473, 1000, 640)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_ROWS)
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_gemm_int8_many_rows(cuda, m, n, k, out_dtype):
+    from rpfq_review_b200 import _lib, ops
+    xq, xs, wq, ws = _operands(cuda, m, n, k, seed=m + n + k)
+    g = torch.Generator().manual_seed(6)
+    bias = torch.randn(n, generator=g).to(cuda)
+    res = torch.randn(m, n, generator=g).to(out_dtype).to(cuda)
+    for b, act, r in ((bias, "none", None), (bias.half(), "gelu", res)):
+        y = ops.gemm_int8(xq, xs, wq, ws, bias=b, residual=r, activation=act, out_dtype=out_dtype)
+        _check(y, _product_ref(xq, xs, wq, ws, b, act, r, out_dtype))
+    # rows that TMA can store but not load and the other way round, in place too
+    wide = torch.full((m, n + 24), 5.0, dtype=out_dtype, device=cuda)
+    want = y
+    for out_off, res_off in ((8, 1), (1, 8)):
+        rv = wide.clone()[:, res_off:res_off + n]
+        rv.copy_(res)
+        buf = wide.clone()
+        out = buf[:, out_off:out_off + n]
+        ops.gemm_int8(xq, xs, wq, ws, bias=bias.half(), residual=rv, activation="gelu", out=out)
+        assert torch.equal(out, want)
+        out.fill_(5.0)
+        assert torch.equal(buf, wide)
+        ops.gemm_int8(xq, xs, wq, ws, bias=bias.half(), residual=rv, activation="gelu", out=rv)
+        assert torch.equal(rv, want)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+
+
 def test_gemm_int8_largest_sums(cuda):
     """k = 131071 codes of -128 reach 2^31 - 2^14: no overflow; one more is refused."""
     from rpfq_review_b200 import ops

@@ -181,11 +181,19 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
  * residual. Requirements: x and w 16-byte aligned with row strides that are
  * multiples of 16 (any k up to 131071 within such rows); y, residual, bias and
  * the scales aligned to their values, any n and any row strides >= n; the
- * residual has y's dtype. Nothing is kept between calls. */
+ * residual has y's dtype. Nothing is kept between calls.
+ * With RPFQ_GEMM_X_F16 or RPFQ_GEMM_X_F32 in flags, x holds fp16 or fp32
+ * activations (any row stride >= k, x_scale unused): their rows are quantized
+ * as by rpfq_quantize_rows_sm100, inside the product's launch for at most 8
+ * rows and into `scratch` otherwise. scratch is device memory, 16-byte
+ * aligned, of at least rpfq_gemm_i8_scratch_bytes(m, k) bytes (NULL where that
+ * is 0); calls that may overlap on the GPU need their own. The result is that
+ * of the two calls, bit for bit. */
+enum { RPFQ_GEMM_X_F16 = 8, RPFQ_GEMM_X_F32 = 16 };
 typedef struct RpfqGemmI8Args {
-    const int8_t* x;          /* int8 [m, k], row stride ldx                            */
+    const void* x;            /* int8 codes [m, k] (fp16 / fp32 by flags), row stride ldx */
     int64_t ldx;
-    const float* x_scale;     /* fp32 [m]                                               */
+    const float* x_scale;     /* fp32 [m] of the codes                                  */
     const int8_t* w;          /* int8 [n, k], row stride ldw                            */
     int64_t ldw;
     const float* w_scale;     /* fp32 [n]                                               */
@@ -197,8 +205,12 @@ typedef struct RpfqGemmI8Args {
     int64_t m;
     int32_t n, k;
     int32_t activation;       /* RPFQ_ACT_NONE or RPFQ_ACT_GELU (erf)                   */
-    int32_t flags;            /* RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32 */
+    int32_t flags;            /* RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32
+                                 | RPFQ_GEMM_X_F16 or RPFQ_GEMM_X_F32                   */
+    void* scratch;            /* codes and scales of quantized activations, or NULL     */
+    uint64_t scratch_bytes;
 } RpfqGemmI8Args;
+uint64_t rpfq_gemm_i8_scratch_bytes(int64_t m, int32_t k);
 int rpfq_gemm_i8_sm100(const RpfqGemmI8Args* args, rpfq_stream_t stream);
 
 enum { RPFQ_POS_I32 = 0, RPFQ_POS_I64 = 1, RPFQ_POS_F32 = 2, RPFQ_POS_F64 = 3 }; /* types of a position */

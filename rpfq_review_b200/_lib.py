@@ -25,6 +25,8 @@ ACT_GELU = 1
 GEMM_OUT_F32 = 1
 GEMM_RESIDUAL_F32 = 2
 GEMM_BIAS_F32 = 4
+GEMM_X_F16 = 8
+GEMM_X_F32 = 16
 POS_I32 = 0
 POS_I64 = 1
 POS_F32 = 2
@@ -40,6 +42,7 @@ EXPORTED_SYMBOLS = (
     "rpfq_gemm_plan_sm100",
     "rpfq_act_quant_sm100",
     "rpfq_quantize_rows_sm100",
+    "rpfq_gemm_i8_scratch_bytes",
     "rpfq_gemm_i8_sm100",
     "rpfq_rotary_sm100",
     "rpfq_patch_unfold_sm100",
@@ -109,6 +112,7 @@ class RpfqGemmI8Args(ctypes.Structure):
         ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
         ("m", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
         ("activation", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64),
     ]
 
 
@@ -185,6 +189,8 @@ def lib() -> ctypes.CDLL:
         L.rpfq_act_quant_sm100.argtypes = [P, I64, P, I64, I64, I32, I32, P]
         L.rpfq_quantize_rows_sm100.argtypes = [P, I32, I64, P, I64, P, I64, I32, P]
         L.rpfq_gemm_i8_sm100.argtypes = [ctypes.POINTER(RpfqGemmI8Args), P]
+        L.rpfq_gemm_i8_scratch_bytes.argtypes = [I64, I32]
+        L.rpfq_gemm_i8_scratch_bytes.restype = ctypes.c_uint64
         L.rpfq_rotary_sm100.argtypes = [ctypes.POINTER(RpfqRotaryArgs), P]
         L.rpfq_patch_unfold_sm100.argtypes = [P, I32, I64, I32, I32, I32, I32, P, I64, P]
         L.rpfq_layernorm_sm100.argtypes = [P, I64, P, P, P, I64, I64, I32, ctypes.c_float, I32, P]

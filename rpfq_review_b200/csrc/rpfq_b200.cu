@@ -16,6 +16,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "../../include/rpfq_b200.h"
 #include "actquant.cuh"
@@ -25,6 +26,7 @@
 #include "embed.cuh"
 #include "gemm.cuh"
 #include "gemm_i8.cuh"
+#include "gemm_i8_few.cuh"
 #include "gemm_i8_pair.cuh"
 #include "layernorm.cuh"
 #include "pack.cuh"
@@ -784,6 +786,41 @@ int gemm(const RpfqGemmArgs* a, cudaStream_t stream, RpfqGemmPlan* dry = nullptr
     return launch_gemm_bn<128, false>(a, st, stream, splits, false, false, dry);
 }
 
+// ---------------------------------------------------------------- row quantizer
+template <typename T>
+cudaError_t launch_quantize_rows(bool vec, bool block_row, int64_t blocks, cudaStream_t stream,
+                                 const QuantizeRowsParams& p) {
+    const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+    if (vec)
+        return block_row ? launch_kernel(quantize_rows_kernel<T, true, 256>, grid, block, 0, stream, 1, p)
+                         : launch_kernel(quantize_rows_kernel<T, true, 32>, grid, block, 0, stream, 1, p);
+    return block_row ? launch_kernel(quantize_rows_kernel<T, false, 256>, grid, block, 0, stream, 1, p)
+                     : launch_kernel(quantize_rows_kernel<T, false, 32>, grid, block, 0, stream, 1, p);
+}
+
+// Checked arguments; the caller has set up the device.
+int quantize_rows(const char* who, const void* x, bool f32, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t m,
+                  int32_t k, DeviceState* st, cudaStream_t stream) {
+    QuantizeRowsParams p;
+    p.x = x;
+    p.ldx = ldx;
+    p.q = q;
+    p.ldq = ldq;
+    p.scale = scale;
+    p.m = m;
+    p.k = k;
+    // a block per row when warps would not fill the GPU or keep the row
+    const int esize = f32 ? 4 : 2;
+    const bool block_row = m < int64_t(8) * st->sm_count || int64_t(k) * esize > 32 * 16 * kQuantRowKeep;
+    const int64_t blocks = block_row ? m : (m + 7) / 8;
+    if (blocks > 0x7fffffff || k > (1 << 30)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or k too large", who);
+    const int qvec = 16 / esize;
+    const bool vec = aligned16(x) && ldx * esize % 16 == 0 && reinterpret_cast<uintptr_t>(q) % qvec == 0 && ldq % qvec == 0;
+    RPFQ_CUDA((f32 ? launch_quantize_rows<float>(vec, block_row, blocks, stream, p)
+                   : launch_quantize_rows<__half>(vec, block_row, blocks, stream, p)));
+    return RPFQ_OK;
+}
+
 // ---------------------------------------------------------------- int8 product
 constexpr int32_t kGemmI8MaxK = 131071;  // 128 * 128 * k < 2^31
 
@@ -880,37 +917,89 @@ bool i8_vec_out(const RpfqGemmI8Args* a) {
     return !a->residual || (reinterpret_cast<uintptr_t>(a->residual) % bytes == 0 && a->ldr % 4 == 0);
 }
 
-int gemm_i8(const RpfqGemmI8Args* a, cudaStream_t stream) {
+// Rows that the few-row kernel takes: their codes lie in its shared memory.
+bool few_rows_fit(int64_t m, int64_t k) { return m <= kFewRows && m * ((k + 15) / 16 * 16) <= kFewSmem; }
+
+template <int ROWS, int COLS, int XT, bool OUT_F32>
+int launch_i8_few(const GemmI8FewParams& p, cudaStream_t stream) {
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t attr_status[kMaxDevices];
+    int dev = 0;
+    RPFQ_CUDA(cudaGetDevice(&dev));
+    std::call_once(once[dev], [dev]() {
+        attr_status[dev] = cudaFuncSetAttribute(gemm_i8_few_kernel<ROWS, COLS, XT, OUT_F32>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    });
+    RPFQ_CUDA(attr_status[dev]);
+    const int per_block = kFewThreads / 32 * COLS;
+    const size_t smem = static_cast<size_t>(p.g.m) * ((p.g.k + 15) / 16 * 16);
+    RPFQ_CUDA((launch_kernel(gemm_i8_few_kernel<ROWS, COLS, XT, OUT_F32>, dim3((p.g.n + per_block - 1) / per_block),
+                             dim3(kFewThreads), smem, stream, 1, p)));
+    return RPFQ_OK;
+}
+
+template <int XT, bool OUT_F32>
+int launch_i8_few_rows(const GemmI8FewParams& p, cudaStream_t stream) {
+    if (p.g.m == 1) return launch_i8_few<1, 1, XT, OUT_F32>(p, stream);
+    if (p.g.m == 2) return launch_i8_few<2, 2, XT, OUT_F32>(p, stream);
+    if (p.g.m <= 4) return launch_i8_few<4, 2, XT, OUT_F32>(p, stream);
+    return launch_i8_few<kFewRows, 4, XT, OUT_F32>(p, stream);
+}
+
+int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     const char* who = "rpfq_gemm_i8_sm100";
-    if (!a) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
+    if (!args) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
+    RpfqGemmI8Args own = *args;
+    const RpfqGemmI8Args* a = &own;
     if (a->m < 0 || a->n <= 0 || a->k <= 0)
         return fail(RPFQ_ERR_INVALID, "%s: bad shape m=%lld n=%d k=%d", who, (long long)a->m, a->n, a->k);
     if (a->k > kGemmI8MaxK)
         return fail(RPFQ_ERR_UNSUPPORTED, "%s: k must be at most %d (int32 sums), got %d", who, kGemmI8MaxK, a->k);
-    if (a->m > (int64_t(1) << 31) - 256) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m too large", who);
-    if (a->flags & ~(RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32))
-        return fail(RPFQ_ERR_INVALID, "%s: unknown flags 0x%x", who, a->flags);
+    if (a->m > (int64_t(1) << 31) - 256 || a->n > 0x7fffffff - 256)
+        return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or n too large", who);
+    const int x_flags = a->flags & (RPFQ_GEMM_X_F16 | RPFQ_GEMM_X_F32);
+    if ((a->flags & ~(RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32 | RPFQ_GEMM_X_F16 | RPFQ_GEMM_X_F32)) ||
+        x_flags == (RPFQ_GEMM_X_F16 | RPFQ_GEMM_X_F32))
+        return fail(RPFQ_ERR_INVALID, "%s: bad flags 0x%x", who, a->flags);
     if (a->activation != RPFQ_ACT_NONE && a->activation != RPFQ_ACT_GELU)
         return fail(RPFQ_ERR_INVALID, "%s: unknown activation %d", who, a->activation);
     if (!a->w || !a->w_scale) return fail(RPFQ_ERR_INVALID, "%s: w and w_scale are required", who);
     if (a->m == 0) return RPFQ_OK;
-    if (!a->x || !a->x_scale || !a->y) return fail(RPFQ_ERR_INVALID, "%s: x, x_scale and y are required", who);
-    if (a->ldx < a->k || a->ldx % 16 || a->ldw < a->k || a->ldw % 16)
-        return fail(RPFQ_ERR_INVALID, "%s: row strides of x and w must be >= k and multiples of 16", who);
-    if (!aligned16(a->x) || !aligned16(a->w)) return fail(RPFQ_ERR_INVALID, "%s: x and w must be 16-byte aligned", who);
+    if (!a->x || (!a->x_scale && !x_flags) || !a->y) return fail(RPFQ_ERR_INVALID, "%s: x, x_scale and y are required", who);
+    if (a->ldx < a->k || a->ldw < a->k || a->ldw % 16 || (!x_flags && a->ldx % 16))
+        return fail(RPFQ_ERR_INVALID, "%s: row strides of x and w must be >= k and (codes) multiples of 16", who);
+    if ((!x_flags && !aligned16(a->x)) || !aligned16(a->w))
+        return fail(RPFQ_ERR_INVALID, "%s: codes must be 16-byte aligned", who);
     if (a->ldy < a->n || (a->residual && a->ldr < a->n))
         return fail(RPFQ_ERR_INVALID, "%s: row strides of y and residual must be >= n", who);
     const uintptr_t esize = (a->flags & RPFQ_GEMM_OUT_F32) ? 4 : 2;
     const uintptr_t bsize = (a->flags & RPFQ_GEMM_BIAS_F32) ? 4 : 2;
+    const uintptr_t xsize = x_flags == RPFQ_GEMM_X_F32 ? 4 : (x_flags ? 2 : 1);
     if (reinterpret_cast<uintptr_t>(a->y) % esize || reinterpret_cast<uintptr_t>(a->residual) % esize ||
-        reinterpret_cast<uintptr_t>(a->bias) % bsize || reinterpret_cast<uintptr_t>(a->x_scale) % 4 ||
-        reinterpret_cast<uintptr_t>(a->w_scale) % 4)
+        reinterpret_cast<uintptr_t>(a->bias) % bsize || reinterpret_cast<uintptr_t>(a->x) % xsize ||
+        reinterpret_cast<uintptr_t>(a->x_scale) % 4 || reinterpret_cast<uintptr_t>(a->w_scale) % 4)
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
     if (a->residual && (((a->flags & RPFQ_GEMM_RESIDUAL_F32) != 0) != ((a->flags & RPFQ_GEMM_OUT_F32) != 0)))
         return fail(RPFQ_ERR_UNSUPPORTED, "%s: the residual must have the output's dtype", who);
+    const bool few = few_rows_fit(a->m, a->k);
+    const uint64_t need = x_flags ? rpfq_gemm_i8_scratch_bytes(a->m, a->k) : 0;
+    if (need && (!a->scratch || !aligned16(a->scratch) || a->scratch_bytes < need))
+        return fail(RPFQ_ERR_INVALID, "%s: quantizing %lld rows needs 16-byte aligned scratch of %llu bytes", who,
+                    (long long)a->m, (unsigned long long)need);
     DeviceState* st;
     int rc = device_state(&st);
     if (rc) return rc;
+    if (need) {
+        // codes [m, round_up(k, 16)], then the scales
+        const int64_t ld = (a->k + 15) / 16 * 16;
+        int8_t* codes = static_cast<int8_t*>(a->scratch);
+        float* scale = reinterpret_cast<float*>(codes + a->m * ld);
+        rc = quantize_rows(who, a->x, xsize == 4, a->ldx, codes, ld, scale, a->m, a->k, st, stream);
+        if (rc) return rc;
+        own.x = codes;
+        own.ldx = ld;
+        own.x_scale = scale;
+    }
     GemmI8Params p;
     p.x_scale = a->x_scale;
     p.w_scale = a->w_scale;
@@ -930,6 +1019,20 @@ int gemm_i8(const RpfqGemmI8Args* a, cudaStream_t stream) {
     p.err = st->err_word;
     const bool f32 = (a->flags & RPFQ_GEMM_OUT_F32) != 0;
     const bool res = a->residual != nullptr;
+    if (few) {
+        GemmI8FewParams fp;
+        fp.g = p;
+        fp.x = a->x;
+        fp.ldx = a->ldx;
+        fp.w = a->w;
+        fp.ldw = a->ldw;
+        fp.x_vector = aligned16(a->x) && a->ldx * static_cast<int64_t>(xsize) % 16 == 0;
+        if (x_flags == RPFQ_GEMM_X_F16)
+            return f32 ? launch_i8_few_rows<kXHalf, true>(fp, stream) : launch_i8_few_rows<kXHalf, false>(fp, stream);
+        if (x_flags)
+            return f32 ? launch_i8_few_rows<kXFloat, true>(fp, stream) : launch_i8_few_rows<kXFloat, false>(fp, stream);
+        return f32 ? launch_i8_few_rows<kXCodes, true>(fp, stream) : launch_i8_few_rows<kXCodes, false>(fp, stream);
+    }
     const int64_t pair_tiles = ((a->m + 255) / 256) * ((a->n + 255) / 256);
     if (pair_tiles >= st->sm_count / 2) {
         const int units = f32 ? (res ? i8_pair_units<true, true>(st) : i8_pair_units<true, false>(st))
@@ -1126,21 +1229,12 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
     DeviceState* st;
     int rc = device_state(&st);
     if (rc) return rc;
-    QuantizeRowsParams p;
-    p.x = x;
-    p.ldx = ldx;
-    p.q = q;
-    p.ldq = ldq;
-    p.scale = scale;
-    p.m = m;
-    p.k = k;
-    const int64_t blocks = (m + 7) / 8;
-    if (blocks > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m too large", who);
-    const dim3 grid(static_cast<unsigned>(blocks));
-    cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    RPFQ_CUDA(x_f32 ? launch_kernel(quantize_rows_kernel<float>, grid, dim3(256), 0, cs, 1, p)
-                    : launch_kernel(quantize_rows_kernel<__half>, grid, dim3(256), 0, cs, 1, p));
-    return RPFQ_OK;
+    return quantize_rows(who, x, x_f32 != 0, ldx, q, ldq, scale, m, k, st, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t rpfq_gemm_i8_scratch_bytes(int64_t m, int32_t k) {
+    if (m <= 0 || k <= 0 || few_rows_fit(m, k)) return 0;
+    return static_cast<uint64_t>(m) * ((k + 15) / 16 * 16 + 4);
 }
 
 int rpfq_gemm_i8_sm100(const RpfqGemmI8Args* args, rpfq_stream_t stream) {

@@ -26,7 +26,8 @@ _ROUND = {"rne": _lib.ROUND_NEAREST_EVEN, "ties_away": _lib.ROUND_TIES_AWAY}
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 class LaunchTimer:
@@ -513,49 +514,47 @@ def _forward_only(name: str, *tensors) -> None:
         raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
 
 
-def _same_device(name: str, device: torch.device, **tensors) -> None:
+def _same_device(name: str, index: int, **tensors) -> None:
     for what, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name}: {what} is on {t.device}, not on {device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name}: {what} is on {t.device}, not on cuda:{index}")
 
 
 def _float_type(t: torch.Tensor, name: str) -> bool:
     """True for float32, False for float16; anything else is refused."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype not in (torch.float16, torch.float32):
-        raise ValueError(f"{name} must be float16 or float32, got {t.dtype}")
-    return t.dtype == torch.float32
+    if t.dtype is torch.float16:
+        return False
+    if t.dtype is torch.float32:
+        return True
+    raise ValueError(f"{name} must be float16 or float32, got {t.dtype}")
+
+
+def _matrix(t: torch.Tensor, k: int, name: str):
+    """``t[..., k]`` as rows: (tensor to keep, rows, row stride)."""
+    if t.dim() == 0 or t.shape[-1] != k:
+        raise ValueError(f"{name}: last dim of {tuple(t.shape)} is not {k}")
+    if t.is_contiguous():
+        return t, t.numel() // k, k
+    t2, ld = _rows(t, k, name)
+    if ld < k:  # rows that overlap (expanded): one copy
+        t2, ld = t2.contiguous(), k
+    return t2, t2.shape[0], ld
 
 
 def _code_rows(q: torch.Tensor, k: int, name: str):
-    """``q[..., k]`` int8 as 2-D rows that start on 16 bytes (what the TMA loads
-    need): rows of another stride or address are copied into such rows."""
-    q2, ld = _rows(q, k, name)
-    rows = q2.shape[0]
+    """``q[..., k]`` int8 as rows that start on 16 bytes (what the TMA loads need):
+    rows of another stride or address are copied into such rows."""
+    q2, rows, ld = _matrix(q, k, name)
     if rows <= 1:
         ld = (k + 15) // 16 * 16
-    if ld < k or ld % 16 or q2.data_ptr() % 16:
+    if ld % 16 or q2.data_ptr() % 16:
         ld = (k + 15) // 16 * 16
         buf = torch.empty((rows, ld), dtype=torch.int8, device=q.device)
-        buf[:, :k] = q2
+        buf[:, :k] = q2.reshape(rows, k)
         q2 = buf
-    return q2, ld
-
-
-def _quantize_rows(x: torch.Tensor, k: int, f32: bool):
-    """Codes [m, ld] (k columns used, rows on 16 bytes) and scales [m] of ``x[..., k]``."""
-    x2, ldx = _rows(x, k, "x")
-    if ldx < k:  # rows that overlap (expanded): one copy
-        x2, ldx = x2.contiguous(), k
-    m, ld = x2.shape[0], (k + 15) // 16 * 16
-    q = torch.empty((m, ld), dtype=torch.int8, device=x.device)
-    scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    _lib.check(_lib.lib().rpfq_quantize_rows_sm100(x2.data_ptr(), int(f32), ldx, q.data_ptr(), ld, scale.data_ptr(),
-                                                   m, k, _stream(x.device)), "rpfq_quantize_rows_sm100")
-    if m:
-        _count_launch()
-    return q, scale, ld
+    return q2, rows, ld
 
 
 def quantize_rows(x: torch.Tensor):
@@ -571,51 +570,70 @@ def quantize_rows(x: torch.Tensor):
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(x.shape)}")
     k = x.shape[-1]
+    x2, m, ldx = _matrix(x, k, "x")
+    ld = (k + 15) // 16 * 16
+    q = torch.empty((m, ld), dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     with torch.cuda.device(x.device):
-        q, scale, ld = _quantize_rows(x, k, f32)
-    if ld == k:
-        return q.view(x.shape), scale.view(x.shape[:-1])
-    codes = q.view(*x.shape[:-1], ld)[..., :k]
-    return codes, scale.view(x.shape[:-1])
+        _lib.check(_lib.lib().rpfq_quantize_rows_sm100(x2.data_ptr(), int(f32), ldx, q.data_ptr(), ld,
+                                                       scale.data_ptr(), m, k, _stream(x.device)),
+                   "rpfq_quantize_rows_sm100")
+    if m:
+        _count_launch()
+    codes = q.view(*x.shape[:-1], ld)
+    return (codes if ld == k else codes[..., :k]), scale
 
 
-def _product_int8(name: str, lead, x_ptr: int, ldx: int, x_scale: torch.Tensor, m: int, w: torch.Tensor,
-                  w_scale: torch.Tensor, bias, residual, activation, out, out_dtype) -> torch.Tensor:
-    """The checks and the launch that gemm_int8 and linear_int8 share."""
+def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x_scale, x_flag: int, w: torch.Tensor,
+               w_scale: torch.Tensor, bias, residual, activation, out, out_dtype) -> torch.Tensor:
+    """What gemm_int8 and linear_int8 share: the checks of everything but x, and the launch."""
+    index = x.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _gemm_int8(name, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
+                              out_dtype)
     n, k = w.shape
-    device = x_scale.device
     _require(w_scale, "w_scale", torch.float32)
     if w_scale.numel() != n:
         raise ValueError(f"{name}: w_scale must hold {n} values, got {w_scale.numel()}")
-    w2, ldw = _code_rows(w, k, "w")
-    w_scale = w_scale.contiguous()
     if activation not in _ACT:
         raise ValueError(f"{name}: unknown activation {activation!r}")
+    bias_ptr = None
     if bias is not None:
         if not bias.is_cuda or bias.numel() != n:
             raise ValueError(f"{name}: bias must be a CUDA tensor of {n} values")
         bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    w2, _, ldw = _code_rows(w, k, "w")
+    w_scale = w_scale.contiguous()
     if out is None:
-        out = torch.empty((*lead, n), dtype=out_dtype, device=device)
-    y2, ldy = _rows(out, n, "out")
-    if y2.data_ptr() != out.data_ptr() or y2.shape[0] != m or (m > 1 and ldy < n):
-        raise ValueError(f"{name}: out must be a row-major view of {m} rows with unit column stride")
-    r2, ldr = (None, 0)
+        out = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=x.device)
+        ldy = n
+    else:
+        y2, rows, ldy = _matrix(out, n, "out")
+        if y2.data_ptr() != out.data_ptr() or rows != m:
+            raise ValueError(f"{name}: out must be a row-major view of {m} rows with unit column stride")
+    r2, ldr, r_ptr = None, 0, None
     if residual is not None:
         if not residual.is_cuda:
-            raise ValueError("residual must be a CUDA tensor")
-        r2, ldr = _rows(residual, n, "residual")
-        if r2.shape[0] != m:
+            raise ValueError(f"{name}: residual must be a CUDA tensor")
+        r2, rows, ldr = _matrix(residual, n, "residual")
+        if rows != m:
             raise ValueError(f"{name}: residual rows do not match x")
-        if ldr < n:
-            r2, ldr = r2.contiguous(), n
-    _same_device(name, device, w=w, w_scale=w_scale, bias=bias, residual=residual, out=out)
-    a = _lib.RpfqGemmI8Args(x=x_ptr, ldx=ldx, x_scale=x_scale.data_ptr(), w=w2.data_ptr(), ldw=ldw,
-                            w_scale=w_scale.data_ptr(), bias=_p(bias), residual=_p(r2), ldr=ldr, y=y2.data_ptr(),
-                            ldy=ldy, m=m, n=n, k=k, activation=_ACT[activation], flags=_flags(out, r2, bias))
-    _lib.check(_lib.lib().rpfq_gemm_i8_sm100(ctypes.byref(a), _stream(device)), "rpfq_gemm_i8_sm100")
+        r_ptr = r2.data_ptr()
+    _same_device(name, index, w=w, w_scale=w_scale, bias=bias, residual=residual, out=out)
+    L = _lib.lib()
+    scratch, need = None, 0
+    if x_flag:
+        need = L.rpfq_gemm_i8_scratch_bytes(m, k)
+        if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+    a = _lib.RpfqGemmI8Args(x2.data_ptr(), ldx, x_scale, w2.data_ptr(), ldw, w_scale.data_ptr(), bias_ptr, r_ptr, ldr,
+                            out.data_ptr(), ldy, m, n, k, _ACT[activation], x_flag | _flags(out, r2, bias),
+                            _p(scratch), need)
+    _lib.check(L.rpfq_gemm_i8_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index)), "rpfq_gemm_i8_sm100")
     if m:
-        _count_launch()
+        _count_launch(2 if need else 1)
     return out
 
 
@@ -640,31 +658,28 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     _check_codes(name, w)
     _require(x_scale, "x_scale", torch.float32)
     _forward_only(name, x_scale, w_scale, residual)
-    _same_device(name, x.device, x_scale=x_scale)
-    with torch.cuda.device(x.device):
-        x2, ldx = _code_rows(x, w.shape[1], "x")
-        m = x2.shape[0]
-        if x_scale.numel() != m:
-            raise ValueError(f"{name}: x_scale must hold one value per row ({m}), got {x_scale.numel()}")
-        return _product_int8(name, x.shape[:-1], x2.data_ptr(), ldx, x_scale.contiguous(), m, w, w_scale, bias,
-                             residual, activation, out, out_dtype)
+    x2, m, ldx = _code_rows(x, w.shape[1], "x")
+    if x_scale.numel() != m:
+        raise ValueError(f"{name}: x_scale must hold one value per row ({m}), got {x_scale.numel()}")
+    _same_device(name, x.get_device(), x_scale=x_scale)
+    x_scale = x_scale.contiguous()
+    return _gemm_int8(name, x, x2, m, ldx, x_scale.data_ptr(), 0, w, w_scale, bias, residual, activation, out,
+                      out_dtype)
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 residual: torch.Tensor | None = None, activation="none", out: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The 8-bit linear layer of fp16 or fp32 activations ``x[..., k]``: the rows
-    of x go through :func:`quantize_rows`, the codes through :func:`gemm_int8`
-    with the weight's codes and scales (``w, w_scale = quantize_rows(weight)``).
-    The other arguments as there."""
+    of x as :func:`quantize_rows` codes them, then :func:`gemm_int8` with the
+    weight's codes and scales (``w, w_scale = quantize_rows(weight)``), the same
+    bits as the two calls. The other arguments as there."""
     name = "linear_int8"
-    f32 = _float_type(x, "x")
+    x_flag = _lib.GEMM_X_F32 if _float_type(x, "x") else _lib.GEMM_X_F16
     _check_codes(name, w)
     _forward_only(name, x, w_scale, residual)
-    with torch.cuda.device(x.device):
-        q, scale, ld = _quantize_rows(x, w.shape[1], f32)
-        return _product_int8(name, x.shape[:-1], q.data_ptr(), ld, scale, q.shape[0], w, w_scale, bias, residual,
-                             activation, out, out_dtype)
+    x2, m, ldx = _matrix(x, w.shape[1], "x")
+    return _gemm_int8(name, x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out, out_dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -773,18 +788,21 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
         raise ValueError(f"{name}: out must be {tuple(x.shape)} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
     elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or (D > 1 and out.stride(-1) != 1):
         raise ValueError(f"{name}: out must not be expanded and must have unit stride inside a head")
-    _same_device(name, x.device, positions=positions, inv_freq=inv_freq, out=out)
+    index = x.get_device()
+    _same_device(name, index, positions=positions, inv_freq=inv_freq, out=out)
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     xs, ys = x.stride(), out.stride()
-    a = _lib.RpfqRotaryArgs(x=x.data_ptr(), x_batch=xs[0] if x.dim() == 4 else 0, x_token=xs[-3], x_head=xs[-2],
-                            y=out.data_ptr(), y_batch=ys[0] if x.dim() == 4 else 0, y_token=ys[-3], y_head=ys[-2],
-                            positions=positions.data_ptr(), position_batch=per_sequence,
-                            inv_freq=inv_freq.data_ptr(), batch=B, length=L, heads=H, dim=D, pairs=pairs, axes=axes,
-                            position_type=_POSITION[positions.dtype], f32=int(f32),
-                            interleaved=int(layout == "interleaved"), transpose=int(bool(transpose)),
-                            magnitude=float(magnitude))
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().rpfq_rotary_sm100(ctypes.byref(a), _stream(x.device)), "rpfq_rotary_sm100")
+    four = len(xs) == 4
+    a = _lib.RpfqRotaryArgs(x.data_ptr(), xs[0] if four else 0, xs[-3], xs[-2], out.data_ptr(), ys[0] if four else 0,
+                            ys[-3], ys[-2], positions.data_ptr(), per_sequence, inv_freq.data_ptr(), B, L, H, D,
+                            pairs, axes, _POSITION[positions.dtype], f32, layout == "interleaved", bool(transpose),
+                            magnitude)
+    if torch.cuda.current_device() == index:
+        rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(rc, "rpfq_rotary_sm100")
     if x.numel():
         _count_launch()
     return out

@@ -307,3 +307,26 @@ def test_packed_layer_int8(cuda, n_c, k_c):
     # near the fp16 layer: 8-bit steps of operands whose largest value is a few times their rms
     ref = PackedPhaseLinear.from_packed(layer, activation="gelu")(x).double()
     assert ((mod(x).double() - ref).norm() / ref.norm()).item() < 0.05
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 5, 1), (1, 1000, 768), (2, 33, 17), (3, 4097, 100), (4, 64, 4096), (5, 31, 257),
+                                   (7, 1000, 1003), (8, 770, 2048), (8, 9, 12288), (8, 20, 12304), (1, 7, 98304), (1, 7, 98320)])
+def test_few_rows_same_bits(cuda, m, n, k):
+    """Few rows run on their own kernel (and quantize inside it); rows of a larger
+    product on the tensor cores: the same bits, for codes, fp16 and fp32."""
+    from rpfq_review_b200 import ops
+    g = torch.Generator().manual_seed(m + n + k)
+    x = torch.randn(40, k, generator=g).to(cuda)
+    w, ws = ops.quantize_rows((torch.randn(n, k, generator=g) * 0.1).to(cuda))
+    bias = torch.randn(n, generator=g).to(cuda)
+    for src in (x, x.half()):
+        xq, xs = ops.quantize_rows(src)
+        for dtype in (torch.float16, torch.float32):
+            res = torch.randn(40, n, generator=g).to(dtype).to(cuda)
+            many = ops.gemm_int8(xq, xs, w, ws, bias, res, "gelu", out_dtype=dtype)
+            few = ops.gemm_int8(xq[3:3 + m], xs[3:3 + m], w, ws, bias, res[3:3 + m], "gelu", out_dtype=dtype)
+            assert torch.equal(few, many[3:3 + m])
+            assert torch.equal(ops.linear_int8(src[3:3 + m], w, ws, bias, res[3:3 + m], "gelu", out_dtype=dtype), few)
+            odd = torch.zeros(m, k + 3, dtype=src.dtype, device=cuda)[:, 1:1 + k]
+            odd.copy_(src[3:3 + m])
+            assert torch.equal(ops.linear_int8(odd, w, ws, bias, res[3:3 + m], "gelu", out_dtype=dtype), few)

@@ -16,7 +16,7 @@ A = 4096  # a 16-byte aligned address; nothing is read
 
 
 def test_struct_sizes():
-    assert ctypes.sizeof(_lib.RpfqGemmI8Args) == 8 * 12 + 4 * 4
+    assert ctypes.sizeof(_lib.RpfqGemmI8Args) == 8 * 12 + 4 * 4 + 8 * 2
     assert ctypes.sizeof(_lib.RpfqRotaryArgs) == 8 * 13 + 4 * 10
 
 
@@ -32,7 +32,9 @@ def _gemm(**kw):
     dict(w_scale=None), dict(ldx=48), dict(ldx=72), dict(ldw=48), dict(ldw=60), dict(x=A + 8), dict(w=A + 1),
     dict(ldy=31), dict(residual=A, ldr=31), dict(y=A + 1), dict(y=A + 2, flags=1), dict(bias=A + 1),
     dict(bias=A + 2, flags=4), dict(residual=A + 1, ldr=32), dict(x_scale=A + 2), dict(w_scale=A + 1),
-    dict(flags=8), dict(activation=2), dict(activation=-1)])
+    dict(flags=32), dict(flags=24), dict(activation=2), dict(activation=-1),
+    dict(flags=8, x=A + 1), dict(flags=16, x=A + 2), dict(flags=8, ldx=59), dict(flags=8, m=9),
+    dict(flags=8, m=9, scratch=A + 4, scratch_bytes=1 << 20), dict(flags=8, m=9, scratch=A, scratch_bytes=9 * 68 - 1)])
 def test_gemm_i8_rejects(bad):
     assert _gemm(**bad) == _lib.RPFQ_ERR_INVALID
     assert _lib.lib().rpfq_last_error()
@@ -44,6 +46,9 @@ def test_gemm_i8_unsupported_and_empty():
     assert _gemm(m=2 ** 31) == _lib.RPFQ_ERR_UNSUPPORTED
     assert _gemm(residual=A, ldr=32, flags=1) == _lib.RPFQ_ERR_UNSUPPORTED  # fp16 residual, fp32 output
     assert _gemm(residual=A, ldr=32, flags=2) == _lib.RPFQ_ERR_UNSUPPORTED
+    # few rows are quantized inside the launch: no scratch
+    assert [_lib.lib().rpfq_gemm_i8_scratch_bytes(m, 60) for m in (0, 1, 8, 9)] == [0, 0, 0, 9 * 68]
+    assert _lib.lib().rpfq_gemm_i8_scratch_bytes(8, 100000) == 8 * 100004
     assert _gemm(m=0, x=None, y=None, x_scale=None) == _lib.RPFQ_OK
     assert _lib.lib().rpfq_gemm_i8_sm100(None, None) == _lib.RPFQ_ERR_INVALID
 

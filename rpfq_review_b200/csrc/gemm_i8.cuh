@@ -31,10 +31,9 @@ struct GemmI8Params {
     int32_t n, k;
     int32_t activation;
     int32_t bias_f32;
-    int32_t vec_out;         // y (and residual) rows take vectors of four values
+    int32_t vec_out;         // y rows (tile kernel: and the residual's) take vectors of four values; pairs: TMA stores
+    int32_t vec_res;         // pairs: residual rows take TMA loads
     int32_t x_rows;          // rows of the x box: 128, or fewer when m is small
-    int32_t tma_out;         // pair kernel: y rows can be stored by TMA
-    int32_t tma_res;         // pair kernel: residual rows can be loaded by TMA
     int32_t tail_tiles;      // pair kernel: last-wave tiles cut into `pieces` column pieces
     int32_t pieces;          // 0: none; else 2 or 4
     int* err;
@@ -54,12 +53,37 @@ struct GemmI8TileCfg {
     static_assert(BM * ROW * 4 <= STAGES * STAGE_BYTES, "the staged tile reuses the ring");
 };
 
+// GELU(v) = v Phi(v) = max(v, 0) - a Phi(-a) with a = |v|, and Phi(-a) = 2^Q(a) for a
+// polynomial Q of degree 8 fitted to log2 Phi(-a) on [0, 5.5] (weighted by
+// Phi(-a)^0.8, iteratively reweighted least squares); Q falls on beyond that. Off by
+// at most 1.3 x 2^-24 |v| with an exact 2^x in fp32 Horner steps. One
+// special-function result per value, where erf by exponential and reciprocal takes
+// two: with those the epilogue of m = 50432, k = 1024, n = 4096 took 205 us.
+// max.NaN keeps a NaN; the clamp at 64 keeps Q finite (GELU(inf) = inf).
+__device__ __forceinline__ void gelu_log_pair(float& v0, float& v1) {
+    const uint64_t na = f2_pack(fmaxf(-fabsf(v0), -64.0f), fmaxf(-fabsf(v1), -64.0f));
+    auto c2 = [](float c) { return f2_pack(c, c); };
+    uint64_t q = f2_fma(na, c2(-2.02745741e-06f), c2(-3.01461678e-05f));
+    q = f2_fma(na, q, c2(-0.00014467015f));
+    q = f2_fma(na, q, c2(0.000230890437f));
+    q = f2_fma(na, q, c2(0.00717717316f));
+    q = f2_fma(na, q, c2(0.0525683947f));
+    q = f2_fma(na, q, c2(-0.459186375f));
+    q = f2_fma(na, q, c2(1.15110767f));
+    q = f2_fma(na, q, c2(-0.99999994f));
+    float q0, q1;
+    f2_unpack(q, q0, q1);
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(v0));
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(v1));
+    f2_unpack(f2_fma(na, f2_pack(ex2_approx(q0), ex2_approx(q1)), f2_pack(v0, v1)), v0, v1);
+}
+
 // The four outputs at (row, col..col + 3), `live` of them inside n.
 template <bool OUT_F32>
 __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int live, float (&v)[4]) {
     if (p.activation == kActGelu) {
-        gelu_erf_pair(v[0], v[1]);
-        gelu_erf_pair(v[2], v[3]);
+        gelu_log_pair(v[0], v[1]);
+        gelu_log_pair(v[2], v[3]);
     }
     if constexpr (OUT_F32) {
         float* y = static_cast<float*>(p.y) + row * p.ldy + col;

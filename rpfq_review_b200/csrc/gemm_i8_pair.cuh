@@ -7,17 +7,25 @@
 // accumulators (2 x 256 columns): the epilogue of one tile runs under the main
 // loop of the next.
 //
-// CTA = 12 warps: warp 0 TMA producer, warp 1 TMEM owner and (leader CTA) MMA
-// issuer, warps 4..11 epilogue, each with the 32 rows of its TMEM lane quarter
-// and one column half of the tile, in steps of 128 bytes of output per row. The
-// scales and the bias of a tile's columns are staged in shared memory once per
-// tile (a thread holds one row, so every lane reads the same column); the sum is
-// converted to fp32, scaled and biased in packed fp32 pairs.
+// Warp 0 TMA producer, warp 1 TMEM owner and (leader CTA) MMA issuer, from warp 4
+// on the epilogue, each warp with the 32 rows of its TMEM lane quarter and one
+// column group of the tile, in steps of 128 bytes of output per row. A thread holds
+// one row, so the scales and biases of a tile's columns are staged in shared memory
+// (loaded one tile ahead, one copy for the four warps of a column group: a copy per
+// warp would cost a stage of the ring); the sum is converted to fp32, scaled and
+// biased in packed fp32 pairs.
+// The accumulator is released as soon as the warp's last part of it is in
+// registers, by an arrival without release semantics: a release waits for the
+// warp's other memory traffic, which the MMA warp does not read.
 //
 // Output and residual steps go through the warp's 128-B-swizzled staging slots by
 // TMA when their addresses and row strides are multiples of 16 bytes, and by
 // row-wise loads and stores of the warp otherwise (n odd). With a residual there
 // are two slots: the next step's residual lands while this one is used.
+//
+// EW: eight epilogue warps, or sixteen for GELU without a residual (two warps per
+// scheduler do not keep up with its two special-function results per value; the
+// price is one stage of the ring).
 //
 // The last wave of tiles, where at most half full, is cut into column pieces
 // (Schedule, gemm.cuh).
@@ -29,35 +37,49 @@
 
 namespace rpfq {
 
-template <bool RES>
+template <bool RES, int EW>
 struct GemmI8PairCfg {
+    static_assert(EW == 8 || (EW == 16 && !RES), "epilogue warps");
     static constexpr int BM = 128;
     static constexpr int BN = 256;
     static constexpr int BK = 128;  // bytes = int8 values: one swizzle row
-    static constexpr int STAGES = RES ? 5 : 6;
     static constexpr int A_BYTES = BM * BK;
     static constexpr int B_BYTES = BN / 2 * BK;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int EPI_WARPS = 8;
+    static constexpr int GROUP_COLS = BN / (EW / 4);  // columns of a warp
     static constexpr int SLOTS = RES ? 2 : 1;
     static constexpr int SLOT_BYTES = 32 * 128;
     static constexpr int COL_BYTES = BN * 2 * 4;  // w_scale and bias of the tile's columns
-    static constexpr int BAR_BYTES = 384;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * SLOTS * SLOT_BYTES + COL_BYTES + BAR_BYTES;
-    static constexpr int THREADS = 384;
-    // bars: full, empty [STAGES], tfull, tempty [2], drain, residual [2 per warp], then two words
-    static_assert((2 * STAGES + 5 + 2 * EPI_WARPS + 1) * 8 <= BAR_BYTES, "barriers");
-    static_assert(SMEM_BYTES <= 232448, "shared memory budget");
-    // 128 x 40 + 256 x 232 registers <= 384 x 168 at launch
-    static_assert(128 * 40 + 256 * 232 <= THREADS * 168, "register split exceeds the launch allocation");
+    static constexpr int BAR_BYTES = 512;
+    static constexpr int OTHER_BYTES = EW * SLOTS * SLOT_BYTES + COL_BYTES + BAR_BYTES;
+    static constexpr int STAGES = (232448 - OTHER_BYTES) / STAGE_BYTES;  // 6; 5 with 16 warps or a residual
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OTHER_BYTES;
+    static constexpr int THREADS = 128 + 32 * EW;
+    // barriers: full, empty [STAGES], tfull, tempty [2], drain, residual [2 per warp]; two words
+    static_assert((2 * STAGES + 5 + 2 * EW + 1) * 8 <= BAR_BYTES, "barriers");
+    // registers per thread: at launch, of warps 0..3 and of the epilogue warps
+    static constexpr int LAUNCH_REGS = EW == 8 ? 168 : 96;
+    static constexpr int REGS_LOW = EW == 8 ? 40 : 24;
+    static constexpr int REGS_HIGH = EW == 8 ? 232 : 112;
+    static_assert(128 * REGS_LOW + 32 * EW * REGS_HIGH <= THREADS * LAUNCH_REGS,
+                  "register split exceeds the launch allocation");
 };
 
-template <bool OUT_F32, bool RES>
-__global__ void __launch_bounds__(384, 1)
+template <int REGS>
+__device__ __forceinline__ void setmaxnreg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS) : "memory");
+}
+template <int REGS>
+__device__ __forceinline__ void setmaxnreg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS) : "memory");
+}
+
+template <bool OUT_F32, bool RES, int EW>
+__global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                         const __grid_constant__ CUtensorMap tm_wp, const __grid_constant__ CUtensorMap tm_y,
                         const __grid_constant__ CUtensorMap tm_r, const GemmI8Params p) {
-    using C = GemmI8PairCfg<RES>;
+    using C = GemmI8PairCfg<RES, EW>;
     constexpr int BN = C::BN;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw;
@@ -66,7 +88,7 @@ __global__ void __launch_bounds__(384, 1)
         return;
     }
     uint8_t* slot_base = smem + C::STAGES * C::STAGE_BYTES;
-    float* col_base = reinterpret_cast<float*>(slot_base + C::EPI_WARPS * C::SLOTS * C::SLOT_BYTES);
+    float* col_base = reinterpret_cast<float*>(slot_base + EW * C::SLOTS * C::SLOT_BYTES);
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(col_base) + C::COL_BYTES);
     uint64_t* full_bar = bars;
     uint64_t* empty_bar = bars + C::STAGES;
@@ -74,10 +96,10 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t* tempty_bar = tfull_bar + 2;
     uint64_t* drain_bar = tfull_bar + 4;
     uint64_t* res_bar = tfull_bar + 5;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_bar + 2 * C::EPI_WARPS);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_bar + 2 * EW);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // uniform
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int num_n = (p.n + BN - 1) / BN;
@@ -95,17 +117,17 @@ __global__ void __launch_bounds__(384, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull_bar[b], 1);
-            mbar_init(&tempty_bar[b], 2 * C::EPI_WARPS);
+            mbar_init(&tempty_bar[b], 2 * EW);
         }
         mbar_init(drain_bar, 1);
-        for (int b = 0; b < 2 * C::EPI_WARPS; ++b) mbar_init(&res_bar[b], 1);
+        for (int b = 0; b < 2 * EW; ++b) mbar_init(&res_bar[b], 1);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&tm_x);
         prefetch_tmap(&tm_w);
         if (p.pieces) prefetch_tmap(&tm_wp);
-        if (p.tma_out) prefetch_tmap(&tm_y);
-        if (RES && p.tma_res) prefetch_tmap(&tm_r);
+        if (p.vec_out) prefetch_tmap(&tm_y);
+        if (RES && p.vec_res) prefetch_tmap(&tm_r);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, 2 * BN);
@@ -120,9 +142,12 @@ __global__ void __launch_bounds__(384, 1)
     pdl_launch_dependents();
 
     if (warp < 4) {
-        setmaxnreg_dec40();
-        if (warp == 0 && lane == 0) {
+        setmaxnreg_dec<C::REGS_LOW>();
+        if (warp == 0) {
             // -------------------------------------------------------- producer
+            const uint32_t elected = elect_one();
+            const uint32_t ring = smem_u32(smem), full0 = smem_u32(full_bar);
+            const uint32_t leader_full0 = mapa_shared(full0, 0);
             int stage = 0;
             uint32_t phase = 0;
             int issued = 0;
@@ -136,16 +161,13 @@ __global__ void __launch_bounds__(384, 1)
                 const int n0 = (w.tile % num_n) * BN + w.n_off + static_cast<int>(rank) * b_rows;
                 const CUtensorMap* tw = w.width == BN ? &tm_w : &tm_wp;
                 for (int kb = 0; kb < num_k; ++kb) {
-                    if (!wait_bar(&empty_bar[stage], phase ^ 1, abort_flag, p.err, 131)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* sa = smem + stage * C::STAGE_BYTES;
+                    ok = __all_sync(0xffffffffu, wait_bar(&empty_bar[stage], phase ^ 1, abort_flag, p.err, 131));
+                    if (!ok) break;
+                    const uint32_t sa = ring + stage * C::STAGE_BYTES;
                     // both CTAs' bytes complete on the leader's barrier
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * bytes);
-                    const uint32_t leader_full = mapa_shared(smem_u32(&full_bar[stage]), 0);
-                    tma_load_2d_pair(sa, &tm_x, leader_full, kb * C::BK, m0);
-                    tma_load_2d_pair(sa + C::A_BYTES, tw, leader_full, kb * C::BK, n0);
+                    if (rank == 0) mbar_arrive_expect_tx_elected(elected, full0 + 8 * stage, 2 * bytes);
+                    tma_load_2d_pair_elected(elected, sa, &tm_x, leader_full0 + 8 * stage, kb * C::BK, m0);
+                    tma_load_2d_pair_elected(elected, sa + C::A_BYTES, tw, leader_full0 + 8 * stage, kb * C::BK, n0);
                     ++issued;
                     if (++stage == C::STAGES) {
                         stage = 0;
@@ -165,13 +187,12 @@ __global__ void __launch_bounds__(384, 1)
                 volatile int no_abort = 0;
                 wait_bar(&full_bar[s], ph, &no_abort, p.err, 132);
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp == 1 && rank == 0) {
             // -------------------------------------------------------- MMA issuer
-            auto commit_both = [&](uint64_t* bar) {
-                const uint32_t a = smem_u32(bar);
-                umma_commit_pair(a);
-                umma_commit_pair(mapa_shared(a, 1));
-            };
+            const uint32_t elected = elect_one();
+            const uint64_t a_desc0 = umma_desc_sw128_kmajor(smem_u32(smem));
+            const uint64_t b_desc0 = umma_desc_sw128_kmajor(smem_u32(smem) + C::A_BYTES);
+            const uint32_t empty0 = smem_u32(empty_bar), tfull0 = smem_u32(tfull_bar);
             int stage = 0;
             uint32_t phase = 0;
             int acc = 0;
@@ -180,58 +201,71 @@ __global__ void __launch_bounds__(384, 1)
             auto sched = schedule();
             WorkItem w;
             while (ok && sched.next(w)) {
-                if (!wait_bar<true>(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.err, 231)) break;
+                ok = __all_sync(0xffffffffu, wait_bar<true>(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.err, 231));
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
                 const uint32_t idesc = umma_idesc_i8(256, w.width);
                 for (int kb = 0; kb < num_k; ++kb) {
-                    if (!wait_bar(&full_bar[stage], phase, abort_flag, p.err, 232)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = __all_sync(0xffffffffu, wait_bar(&full_bar[stage], phase, abort_flag, p.err, 232));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(smem + stage * C::STAGE_BYTES);
-                    const uint64_t a_desc = umma_desc_sw128_kmajor(a_addr);
-                    const uint64_t b_desc = umma_desc_sw128_kmajor(a_addr + C::A_BYTES);
+                    const uint64_t at = static_cast<uint64_t>(stage * (C::STAGE_BYTES >> 4));
 #pragma unroll
                     for (int kk = 0; kk < C::BK / 32; ++kk)
-                        umma_i8_pair(d_tmem, a_desc + 2 * kk, b_desc + 2 * kk, idesc, kb + kk != 0);
-                    commit_both(&empty_bar[stage]);
+                        umma_i8_pair_elected(elected, d_tmem, a_desc0 + at + 2 * kk, b_desc0 + at + 2 * kk, idesc,
+                                             kb + kk != 0);
+                    umma_commit_both_elected(elected, empty0 + 8 * stage);
                     if (++stage == C::STAGES) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
                 if (!ok) break;
-                commit_both(&tfull_bar[acc]);
+                umma_commit_both_elected(elected, tfull0 + 8 * acc);
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1;
                 }
             }
             // no MMA still writes TMEM when it is freed
-            umma_commit_pair(smem_u32(drain_bar));
+            if (elected) umma_commit_pair(smem_u32(drain_bar));
+            __syncwarp();
             volatile int no_abort = 0;
             wait_bar(drain_bar, 0, &no_abort, p.err, 233);
         }
     } else {
-        setmaxnreg_inc232();
+        setmaxnreg_inc<C::REGS_HIGH>();
         // ------------------------------------------------------------ epilogue
-        constexpr int CW = OUT_F32 ? 32 : 64;  // output columns of a step: 128 bytes per row
         constexpr int ESZ = OUT_F32 ? 4 : 2;
-        constexpr int HALF = BN / 2;
+        constexpr int CW = 128 / ESZ;  // output columns of a step
+        constexpr int PER = 16 / ESZ;  // values of a 16-byte granule
+        constexpr int GC = C::GROUP_COLS;
+        using Out = typename std::conditional<OUT_F32, float, __half>::type;
         const int q = warp & 3;
         const int ew = warp - 4;
-        const int col_half = ew >> 2;
+        const int group = ew >> 2;
         uint8_t* slots = slot_base + ew * C::SLOTS * C::SLOT_BYTES;
-        float* s_ws = col_base + col_half * 2 * HALF;  // [HALF] scales, then [HALF] biases
-        float* s_b = s_ws + HALF;
-        const int my_col = threadIdx.x & (HALF - 1);  // the column this thread stages (128 threads per half)
+        float* s_ws = col_base + group * 2 * GC;  // [GC] scales, then [GC] biases
+        float* s_b = s_ws + GC;
+        const int my_col = threadIdx.x & 127;  // the column that this thread stages, if below GC
+        float ws, bias, xs;                    // of the next tile
+        auto load_columns = [&](const WorkItem& w) {
+            const int c = (w.tile % num_n) * BN + w.n_off + group * GC + my_col;
+            const int64_t row = static_cast<int64_t>(w.tile / num_n) * 256 + static_cast<int64_t>(rank) * C::BM + 32 * q + lane;
+            const bool live = my_col < GC && c < p.n;
+            ws = live ? __ldg(p.w_scale + c) : 0.0f;
+            bias = 0.0f;
+            if (p.bias != nullptr && live)
+                bias = p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + c)
+                                  : __half2float(static_cast<const __half*>(p.bias)[c]);
+            xs = row < p.m ? __ldg(p.x_scale + row) : 0.0f;
+        };
         int acc = 0;
         uint32_t acc_phase = 0;
         uint32_t j = 0;      // running step counter of this warp (slot = j & 1 with a residual)
         uint32_t loads = 0;  // residual steps requested (lane 0)
-        bool ok = true;      // after a wait that gave up: only the warps' named barriers are kept up
+        bool ok = true;  // after a wait that gave up: only the warps' named barriers are kept up
         auto load_residual = [&](int s, int col0, int64_t row0) {
             mbar_arrive_expect_tx(&res_bar[2 * ew + s], C::SLOT_BYTES);
             tma_load_2d(slots + s * C::SLOT_BYTES, &tm_r, &res_bar[2 * ew + s], col0, static_cast<int32_t>(row0));
@@ -240,137 +274,151 @@ __global__ void __launch_bounds__(384, 1)
         const uint32_t tempty_leader0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
         const uint32_t tempty_leader1 = mapa_shared(smem_u32(&tempty_bar[1]), 0);
         auto sched = schedule();
-        WorkItem w;
-        while (sched.next(w)) {
+        WorkItem w, next;
+        bool more = sched.next(w);
+        if (more) load_columns(w);
+        while (more) {
             const int64_t row0 = static_cast<int64_t>(w.tile / num_n) * 256 + static_cast<int64_t>(rank) * C::BM + 32 * q;
-            // a piece (width <= HALF) is drained by the first column half's warps
-            const bool piece = w.width != BN;
-            const int c_begin = (w.tile % num_n) * BN + w.n_off + (piece ? 0 : col_half * HALF);
-            const int valid = piece ? (col_half == 0 ? min(w.width, p.n - c_begin) : 0) : min(HALF, p.n - c_begin);
+            const int c_begin = (w.tile % num_n) * BN + w.n_off + group * GC;
+            const int valid = min(min(GC, w.width - group * GC), p.n - c_begin);  // <= 0: past a piece or past n
             const int nsteps = (valid > 0 && row0 < p.m) ? (valid + CW - 1) / CW : 0;
-            const float xs = row0 + lane < p.m ? __ldg(p.x_scale + row0 + lane) : 0.0f;
-            float ws = 0.0f, bias = 0.0f;
-            if (my_col < valid) {
-                ws = __ldg(p.w_scale + c_begin + my_col);
-                if (p.bias != nullptr)
-                    bias = p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + c_begin + my_col)
-                                      : __half2float(static_cast<const __half*>(p.bias)[c_begin + my_col]);
-            }
+            const int rows_live = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
             if constexpr (RES) {
                 // the first residual step lands while the main loop runs
-                if (ok && p.tma_res && lane == 0 && nsteps > 0) {
+                if (ok && p.vec_res && lane == 0 && nsteps > 0) {
                     bulk_wait_group_read<0>();
                     load_residual(j & 1, c_begin, row0);
                 }
             }
-            named_bar_sync(1 + col_half, 128);  // the four warps are done with the previous tile's columns
-            s_ws[my_col] = ws;
-            s_b[my_col] = bias;
-            named_bar_sync(1 + col_half, 128);
-            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(32 * q) << 16) +
-                                   static_cast<uint32_t>(acc * BN + (piece ? 0 : col_half * HALF));
-            if (ok) ok = __all_sync(0xffffffffu, wait_bar(&tfull_bar[acc], acc_phase, abort_flag, p.err, 331));
-            if (!ok) continue;
-            tc_fence_after();
+            named_bar_sync(1 + group, 128);  // the four warps are done with the previous tile's columns
+            if (my_col < GC) {
+                s_ws[my_col] = ws;
+                s_b[my_col] = bias;
+            }
             const uint64_t xs2 = f2_pack(xs, xs);
-            const int rows_live = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;
+            named_bar_sync(1 + group, 128);
+            more = sched.next(next);
+            if (more) load_columns(next);
+            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(32 * q) << 16) +
+                                   static_cast<uint32_t>(acc * BN + group * GC);
+            if (ok) ok = __all_sync(0xffffffffu, wait_bar(&tfull_bar[acc], acc_phase, abort_flag, p.err, 331));
+            if (!ok) {
+                w = next;
+                continue;
+            }
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < nsteps; ++c, ++j) {
                 const int col0 = c_begin + c * CW;
+                const int cols = min(CW, p.n - col0);
                 const uint32_t slot = RES ? (j & 1) : 0;
                 uint8_t* buf = slots + slot * C::SLOT_BYTES;
+                // granule g of row r lives at g ^ (r & 7): the TMA maps' 128-byte swizzle
+                auto granule = [&](int r, int g) { return reinterpret_cast<uint4*>(buf + r * 128 + ((g ^ (r & 7)) << 4)); };
+                auto value = [&](int r, int c) { return reinterpret_cast<Out*>(granule(r, c / PER)) + c % PER; };
                 if constexpr (RES) {
-                    if (p.tma_res) {
+                    if (p.vec_res) {
                         // the next step's residual, once that slot's last store has been read out
                         if (lane == 0 && c + 1 < nsteps) {
                             bulk_wait_group_read<0>();
                             load_residual((j + 1) & 1, col0 + CW, row0);
                         }
                     } else {
-                        if (p.tma_out && lane == 0) bulk_wait_group_read<0>();
+                        if (lane == 0) bulk_wait_group_read<0>();
                         __syncwarp();
-                        const int cols = min(CW, p.n - col0);
-                        for (int r = 0; r < rows_live; ++r)
-                            for (int cc = lane; cc < cols; cc += 32) {
-                                uint8_t* d = buf + r * 128 + (((cc * ESZ >> 4) ^ (r & 7)) << 4) + (cc * ESZ & 15);
-                                const int64_t at = (row0 + r) * p.ldr + col0 + cc;
-                                if constexpr (OUT_F32)
-                                    *reinterpret_cast<float*>(d) = static_cast<const float*>(p.residual)[at];
-                                else
-                                    *reinterpret_cast<__half*>(d) = static_cast<const __half*>(p.residual)[at];
-                            }
-                        __syncwarp();
-                    }
-                }
-                uint32_t r[CW];
+                        const Out* src = static_cast<const Out*>(p.residual) + row0 * p.ldr + col0;
+                        for (int r = 0; r < rows_live; r += 8) {  // eight rows in flight
+                            Out t[8][CW / 32];
 #pragma unroll
-                for (int h = 0; h < CW / 32; ++h)
-                    tmem_ld_32x32b_x32(t_row + c * CW + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * h]));
-                tmem_ld_wait();
-                float v[CW];
+                            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int g = 0; g < CW / 4; ++g) {
-                    const float4 sw = *reinterpret_cast<const float4*>(s_ws + c * CW + 4 * g);
-                    const float4 sb = *reinterpret_cast<const float4*>(s_b + c * CW + 4 * g);
-                    const uint64_t a0 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g])),
-                                                __int2float_rn(static_cast<int>(r[4 * g + 1])));
-                    const uint64_t a1 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g + 2])),
-                                                __int2float_rn(static_cast<int>(r[4 * g + 3])));
-                    f2_unpack(f2_fma(f2_mul(a0, f2_pack(sw.x, sw.y)), xs2, f2_pack(sb.x, sb.y)), v[4 * g], v[4 * g + 1]);
-                    f2_unpack(f2_fma(f2_mul(a1, f2_pack(sw.z, sw.w)), xs2, f2_pack(sb.z, sb.w)), v[4 * g + 2],
-                              v[4 * g + 3]);
-                }
-                if (p.activation == kActGelu) {
+                                for (int cc = 0; cc < CW / 32; ++cc)
+                                    if (r + i < rows_live && 32 * cc + lane < cols)
+                                        t[i][cc] = src[(r + i) * p.ldr + 32 * cc + lane];
 #pragma unroll
-                    for (int jj = 0; jj < CW; jj += 2) gelu_erf_pair(v[jj], v[jj + 1]);
-                }
-                if constexpr (RES) {
-                    if (p.tma_res)
-                        ok = __all_sync(0xffffffffu,
-                                        wait_bar(&res_bar[2 * ew + slot], (j >> 1) & 1, abort_flag, p.err, 332));
-                    if (!ok) break;
-                    // this thread's row of the residual step (128-B swizzle)
+                            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const uint4 rv = *reinterpret_cast<const uint4*>(buf + lane * 128 + ((g ^ (lane & 7)) << 4));
-                        if constexpr (OUT_F32) {
-                            v[4 * g + 0] += __uint_as_float(rv.x);
-                            v[4 * g + 1] += __uint_as_float(rv.y);
-                            v[4 * g + 2] += __uint_as_float(rv.z);
-                            v[4 * g + 3] += __uint_as_float(rv.w);
-                        } else {
-                            const __half2* rh = reinterpret_cast<const __half2*>(&rv);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 f = __half22float2(rh[e]);
-                                v[8 * g + 2 * e] += f.x;
-                                v[8 * g + 2 * e + 1] += f.y;
-                            }
+                                for (int cc = 0; cc < CW / 32; ++cc)
+                                    if (r + i < rows_live && 32 * cc + lane < cols) *value(r + i, 32 * cc + lane) = t[i][cc];
                         }
+                        __syncwarp();
                     }
-                    __syncwarp();  // every lane has read its row before any lane overwrites the slot
                 } else {
                     // single slot: the previous step has left it
-                    if (p.tma_out && lane == 0) bulk_wait_group_read<0>();
+                    if (lane == 0) bulk_wait_group_read<0>();
                     __syncwarp();
                 }
+                // 32 columns at a time; a thread reads and writes its own row of the slot only
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    uint4 pk;
-                    if constexpr (OUT_F32) {
-                        pk = make_uint4(__float_as_uint(v[4 * g]), __float_as_uint(v[4 * g + 1]),
-                                        __float_as_uint(v[4 * g + 2]), __float_as_uint(v[4 * g + 3]));
-                    } else {
-                        const __half2 h0 = __floats2half2_rn(v[8 * g + 0], v[8 * g + 1]);
-                        const __half2 h1 = __floats2half2_rn(v[8 * g + 2], v[8 * g + 3]);
-                        const __half2 h2 = __floats2half2_rn(v[8 * g + 4], v[8 * g + 5]);
-                        const __half2 h3 = __floats2half2_rn(v[8 * g + 6], v[8 * g + 7]);
-                        pk = make_uint4(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1),
-                                        *reinterpret_cast<const uint32_t*>(&h2), *reinterpret_cast<const uint32_t*>(&h3));
+                for (int h = 0; h < CW / 32; ++h) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(t_row + c * CW + 32 * h, r);
+                    tmem_ld_wait(r);
+                    if (c + 1 == nsteps && h + 1 == CW / 32) {
+                        // this warp has read its part of the accumulator into registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(acc ? tempty_leader1 : tempty_leader0);
                     }
-                    *reinterpret_cast<uint4*>(buf + lane * 128 + ((g ^ (lane & 7)) << 4)) = pk;
+                    float v[32];
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const float4 sw = *reinterpret_cast<const float4*>(s_ws + c * CW + 32 * h + 4 * g);
+                        const float4 sb = *reinterpret_cast<const float4*>(s_b + c * CW + 32 * h + 4 * g);
+                        const uint64_t a0 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g])),
+                                                    __int2float_rn(static_cast<int>(r[4 * g + 1])));
+                        const uint64_t a1 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g + 2])),
+                                                    __int2float_rn(static_cast<int>(r[4 * g + 3])));
+                        f2_unpack(f2_fma(f2_mul(a0, f2_pack(sw.x, sw.y)), xs2, f2_pack(sb.x, sb.y)), v[4 * g],
+                                  v[4 * g + 1]);
+                        f2_unpack(f2_fma(f2_mul(a1, f2_pack(sw.z, sw.w)), xs2, f2_pack(sb.z, sb.w)), v[4 * g + 2],
+                                  v[4 * g + 3]);
+                    }
+                    if (p.activation == kActGelu) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) gelu_log_pair(v[e], v[e + 1]);
+                    }
+                    if constexpr (RES) {
+                        if (h == 0 && p.vec_res) {
+                            ok = __all_sync(0xffffffffu,
+                                            wait_bar(&res_bar[2 * ew + slot], (j >> 1) & 1, abort_flag, p.err, 332));
+                            if (!ok) break;
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < 32 / PER; ++g) {
+                        uint4* at = granule(lane, h * (32 / PER) + g);
+                        float* e = v + PER * g;
+                        if constexpr (RES) {
+                            const uint4 a = *at;
+                            if constexpr (OUT_F32) {
+                                e[0] += __uint_as_float(a.x);
+                                e[1] += __uint_as_float(a.y);
+                                e[2] += __uint_as_float(a.z);
+                                e[3] += __uint_as_float(a.w);
+                            } else {
+                                const __half2* rh = reinterpret_cast<const __half2*>(&a);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float2 f = __half22float2(rh[i]);
+                                    e[2 * i] += f.x;
+                                    e[2 * i + 1] += f.y;
+                                }
+                            }
+                        }
+                        if constexpr (OUT_F32) {
+                            *at = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]),
+                                             __float_as_uint(e[3]));
+                        } else {
+                            const __half2 h0 = __floats2half2_rn(e[0], e[1]), h1 = __floats2half2_rn(e[2], e[3]);
+                            const __half2 h2 = __floats2half2_rn(e[4], e[5]), h3 = __floats2half2_rn(e[6], e[7]);
+                            *at = make_uint4(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1),
+                                             *reinterpret_cast<const uint32_t*>(&h2), *reinterpret_cast<const uint32_t*>(&h3));
+                        }
+                    }
                 }
-                if (p.tma_out) {
+                if (!ok) break;
+                if (p.vec_out) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -379,29 +427,35 @@ __global__ void __launch_bounds__(384, 1)
                     }
                 } else {
                     __syncwarp();
-                    const int cols = min(CW, p.n - col0);
-                    for (int r2 = 0; r2 < rows_live; ++r2)
-                        for (int cc = lane; cc < cols; cc += 32) {
-                            const uint8_t* d = buf + r2 * 128 + (((cc * ESZ >> 4) ^ (r2 & 7)) << 4) + (cc * ESZ & 15);
-                            const int64_t at = (row0 + r2) * p.ldy + col0 + cc;
-                            if constexpr (OUT_F32)
-                                static_cast<float*>(p.y)[at] = *reinterpret_cast<const float*>(d);
-                            else
-                                static_cast<__half*>(p.y)[at] = *reinterpret_cast<const __half*>(d);
-                        }
+                    Out* dst = static_cast<Out*>(p.y) + row0 * p.ldy + col0;
+                    for (int r = 0; r < rows_live; r += 8) {
+                        Out t[8][CW / 32];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int cc = 0; cc < CW / 32; ++cc) t[i][cc] = *value(r + i, 32 * cc + lane);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int cc = 0; cc < CW / 32; ++cc)
+                                if (r + i < rows_live && 32 * cc + lane < cols)
+                                    dst[(r + i) * p.ldy + 32 * cc + lane] = t[i][cc];
+                    }
                     __syncwarp();
                     // the next residual may reach this slot by TMA: order these reads before it
-                    if (RES && p.tma_res) fence_proxy_async_smem();
+                    if (RES && p.vec_res) fence_proxy_async_smem();
                 }
             }
-            if (!ok) continue;
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc ? tempty_leader1 : tempty_leader0);
+            if (ok && nsteps == 0) {  // nothing to read: release the accumulator all the same
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(acc ? tempty_leader1 : tempty_leader0);
+            }
             if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1;
             }
+            w = next;
         }
         if (lane == 0) {
             bulk_wait_group<0>();

@@ -848,15 +848,15 @@ int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t 
 }
 
 // Co-resident CTA pairs of the int8 pair kernel (queried once per device and variant; 0 on error).
-template <bool OUT_F32, bool RES>
+template <bool OUT_F32, bool RES, int EW>
 int i8_pair_units(DeviceState* st) {
-    using C = GemmI8PairCfg<RES>;
+    using C = GemmI8PairCfg<RES, EW>;
     static std::once_flag once[kMaxDevices];
     static int units[kMaxDevices] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
     std::call_once(once[dev], [dev, st]() {
-        if (cudaFuncSetAttribute(gemm_i8_pair_kernel<OUT_F32, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(gemm_i8_pair_kernel<OUT_F32, RES, EW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  C::SMEM_BYTES) != cudaSuccess) {
             cudaGetLastError();
             return;
@@ -873,7 +873,7 @@ int i8_pair_units(DeviceState* st) {
         q.attrs = qa;
         q.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<OUT_F32, RES>, &q) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<OUT_F32, RES, EW>, &q) != cudaSuccess) {
             cudaGetLastError();
             return;
         }
@@ -882,30 +882,32 @@ int i8_pair_units(DeviceState* st) {
     return units[dev];
 }
 
-template <bool OUT_F32, bool RES>
-int launch_i8_pair(const RpfqGemmI8Args* a, GemmI8Params p, int units, cudaStream_t stream) {
-    using C = GemmI8PairCfg<RES>;
+template <bool OUT_F32, bool RES, int EW>
+int launch_i8_pair(const RpfqGemmI8Args* a, GemmI8Params p, DeviceState* st, cudaStream_t stream) {
+    const int units = i8_pair_units<OUT_F32, RES, EW>(st);
+    if (units <= 0) return fail(RPFQ_ERR_CUDA, "rpfq_gemm_i8_sm100: occupancy query for CTA pairs failed");
+    using C = GemmI8PairCfg<RES, EW>;
     constexpr int ESZ = OUT_F32 ? 4 : 2;
     constexpr int CW = 128 / ESZ;
     const int64_t tiles = ((a->m + 255) / 256) * ((a->n + 255) / 256);
     if (tiles > 0x7fffffff - units) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
     p.pieces = narrow_pieces(tiles, units);
     p.tail_tiles = p.pieces ? static_cast<int32_t>(tiles % units) : 0;
-    p.tma_out = aligned16(a->y) && a->ldy * ESZ % 16 == 0;
-    p.tma_res = a->residual && aligned16(a->residual) && a->ldr * ESZ % 16 == 0;
+    p.vec_out = aligned16(a->y) && a->ldy * ESZ % 16 == 0;
+    p.vec_res = a->residual && aligned16(a->residual) && a->ldr * ESZ % 16 == 0;
     CUtensorMap tx, tw, twp, ty, tr;
     int rc = make_tmap_i8(&tx, a->x, a->m, a->k, a->ldx, C::BM);
     if (!rc) rc = make_tmap_i8(&tw, a->w, a->n, a->k, a->ldw, C::BN / 2);
     if (!rc && p.pieces) rc = make_tmap_i8(&twp, a->w, a->n, a->k, a->ldw, C::BN / 2 / p.pieces);
-    if (!rc && p.tma_out) rc = make_tmap_f16(&ty, a->y, a->m, a->n, a->ldy, 32, CW, ESZ);
-    if (!rc && p.tma_res) rc = make_tmap_f16(&tr, a->residual, a->m, a->n, a->ldr, 32, CW, ESZ);
+    if (!rc && p.vec_out) rc = make_tmap_f16(&ty, a->y, a->m, a->n, a->ldy, 32, CW, ESZ);
+    if (!rc && p.vec_res) rc = make_tmap_f16(&tr, a->residual, a->m, a->n, a->ldr, 32, CW, ESZ);
     if (rc) return rc;
     // maps that this call does not use
     if (!p.pieces) twp = tw;
-    if (!p.tma_out) ty = tx;
-    if (!p.tma_res) tr = tx;
+    if (!p.vec_out) ty = tx;
+    if (!p.vec_res) tr = tx;
     const int grid = 2 * static_cast<int>(std::min<int64_t>(tiles, units));
-    RPFQ_CUDA((launch_kernel(gemm_i8_pair_kernel<OUT_F32, RES>, dim3(grid), dim3(C::THREADS), C::SMEM_BYTES, stream, 2,
+    RPFQ_CUDA((launch_kernel(gemm_i8_pair_kernel<OUT_F32, RES, EW>, dim3(grid), dim3(C::THREADS), C::SMEM_BYTES, stream, 2,
                              tx, tw, twp, ty, tr, p)));
     return RPFQ_OK;
 }
@@ -1015,7 +1017,7 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     p.bias_f32 = (a->flags & RPFQ_GEMM_BIAS_F32) ? 1 : 0;
     p.vec_out = i8_vec_out(a) ? 1 : 0;
     p.x_rows = a->m >= 128 ? 128 : static_cast<int32_t>((a->m + 7) / 8 * 8);
-    p.tma_out = p.tma_res = p.tail_tiles = p.pieces = 0;
+    p.vec_res = p.tail_tiles = p.pieces = 0;
     p.err = st->err_word;
     const bool f32 = (a->flags & RPFQ_GEMM_OUT_F32) != 0;
     const bool res = a->residual != nullptr;
@@ -1035,12 +1037,10 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     }
     const int64_t pair_tiles = ((a->m + 255) / 256) * ((a->n + 255) / 256);
     if (pair_tiles >= st->sm_count / 2) {
-        const int units = f32 ? (res ? i8_pair_units<true, true>(st) : i8_pair_units<true, false>(st))
-                              : (res ? i8_pair_units<false, true>(st) : i8_pair_units<false, false>(st));
-        if (units <= 0) return fail(RPFQ_ERR_CUDA, "%s: occupancy query for CTA pairs failed", who);
-        if (f32)
-            return res ? launch_i8_pair<true, true>(a, p, units, stream) : launch_i8_pair<true, false>(a, p, units, stream);
-        return res ? launch_i8_pair<false, true>(a, p, units, stream) : launch_i8_pair<false, false>(a, p, units, stream);
+        if (res) return f32 ? launch_i8_pair<true, true, 8>(a, p, st, stream) : launch_i8_pair<false, true, 8>(a, p, st, stream);
+        if (p.activation == RPFQ_ACT_GELU)
+            return f32 ? launch_i8_pair<true, false, 16>(a, p, st, stream) : launch_i8_pair<false, false, 16>(a, p, st, stream);
+        return f32 ? launch_i8_pair<true, false, 8>(a, p, st, stream) : launch_i8_pair<false, false, 8>(a, p, st, stream);
     }
     return (a->flags & RPFQ_GEMM_OUT_F32) ? launch_i8_tile<128, true>(a, p, stream)
                                           : launch_i8_tile<128, false>(a, p, stream);

@@ -301,6 +301,19 @@ __global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
             if (more) load_columns(next);
             const uint32_t t_row = tmem_base + (static_cast<uint32_t>(32 * q) << 16) +
                                    static_cast<uint32_t>(acc * BN + group * GC);
+            // residual rows that TMA cannot load: a step ahead in registers, 32 rows in flight
+            Out rv[RES ? 32 : 1][CW / 32];
+            auto fetch_residual = [&](int c) {
+                const Out* src = static_cast<const Out*>(p.residual) + row0 * p.ldr + c_begin + c * CW + lane;
+#pragma unroll
+                for (int r = 0; r < (RES ? 32 : 1); ++r)
+#pragma unroll
+                    for (int cc = 0; cc < CW / 32; ++cc)
+                        if (r < rows_live && c_begin + c * CW + 32 * cc + lane < p.n) rv[r][cc] = src[r * p.ldr + 32 * cc];
+            };
+            if constexpr (RES) {
+                if (!p.vec_res && nsteps > 0) fetch_residual(0);
+            }
             if (ok) ok = __all_sync(0xffffffffu, wait_bar(&tfull_bar[acc], acc_phase, abort_flag, p.err, 331));
             if (!ok) {
                 w = next;
@@ -326,21 +339,11 @@ __global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
                     } else {
                         if (lane == 0) bulk_wait_group_read<0>();
                         __syncwarp();
-                        const Out* src = static_cast<const Out*>(p.residual) + row0 * p.ldr + col0;
-                        for (int r = 0; r < rows_live; r += 8) {  // eight rows in flight
-                            Out t[8][CW / 32];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
+                        for (int r = 0; r < 32; ++r)
 #pragma unroll
-                                for (int cc = 0; cc < CW / 32; ++cc)
-                                    if (r + i < rows_live && 32 * cc + lane < cols)
-                                        t[i][cc] = src[(r + i) * p.ldr + 32 * cc + lane];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                                for (int cc = 0; cc < CW / 32; ++cc)
-                                    if (r + i < rows_live && 32 * cc + lane < cols) *value(r + i, 32 * cc + lane) = t[i][cc];
-                        }
+                            for (int cc = 0; cc < CW / 32; ++cc) *value(r, 32 * cc + lane) = rv[r][cc];
+                        if (c + 1 < nsteps) fetch_residual(c + 1);
                         __syncwarp();
                     }
                 } else {

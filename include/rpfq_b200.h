@@ -187,8 +187,10 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
  * as by rpfq_quantize_rows_sm100, inside the product's launch for at most 8
  * rows and into `scratch` otherwise. scratch is device memory, 16-byte
  * aligned, of at least rpfq_gemm_i8_scratch_bytes(m, k) bytes (NULL where that
- * is 0); calls that may overlap on the GPU need their own. The result is that
- * of the two calls, bit for bit. */
+ * is 0; with block_n or split_k given, m * (round_up(k, 16) + 4)); calls that
+ * may overlap on the GPU need their own. The result is that of the two calls,
+ * bit for bit, and does not depend on block_n and split_k either: the sums are
+ * exact. */
 enum { RPFQ_GEMM_X_F16 = 8, RPFQ_GEMM_X_F32 = 16 };
 typedef struct RpfqGemmI8Args {
     const void* x;            /* int8 codes [m, k] (fp16 / fp32 by flags), row stride ldx */
@@ -207,6 +209,9 @@ typedef struct RpfqGemmI8Args {
     int32_t activation;       /* RPFQ_ACT_NONE or RPFQ_ACT_GELU (erf)                   */
     int32_t flags;            /* RPFQ_GEMM_OUT_F32 | RPFQ_GEMM_RESIDUAL_F32 | RPFQ_GEMM_BIAS_F32
                                  | RPFQ_GEMM_X_F16 or RPFQ_GEMM_X_F32                   */
+    int32_t block_n;          /* 0 = automatic; else 64 or 128 (one tile per cluster of split_k
+                                 CTAs) or 256 (CTA pairs)                               */
+    int32_t split_k;          /* 0 = automatic; 1..8 = that many k parts per tile       */
     void* scratch;            /* codes and scales of quantized activations, or NULL     */
     uint64_t scratch_bytes;
 } RpfqGemmI8Args;

@@ -112,6 +112,7 @@ class RpfqGemmI8Args(ctypes.Structure):
         ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
         ("m", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
         ("activation", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("block_n", ctypes.c_int32), ("split_k", ctypes.c_int32),
         ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64),
     ]
 

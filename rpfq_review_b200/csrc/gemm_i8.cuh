@@ -7,11 +7,14 @@
 // keeps |sum| < 2^31. The sum is rounded to fp32 once and scaled there; y and
 // residual are fp16 or fp32 (same dtype), rounded once at the end.
 //
-// Tile kernel: one CTA per 128 x BN tile. Warp 0 loads k-blocks of 128 bytes of
-// x and w by TMA (128-byte swizzle) into a ring, warp 1 issues the MMAs into
-// BN TMEM columns; then all six warps move the accumulator through shared memory
-// and write whole rows, lane = column, so any n, stride and alignment is
-// written in order.
+// Tile kernel (fewer rows than fill the GPU with CTA pairs): a cluster of S CTAs
+// per 128 x BN tile, each with every S-th part of the k-blocks. Warp 0 loads
+// k-blocks of 128 bytes of x and w by TMA (128-byte swizzle) into a ring, warp 1
+// issues the MMAs into BN TMEM columns; then all eight warps move the int32 sums to
+// shared memory. With S > 1 CTA r of the cluster adds up the S parts of its share of
+// the rows over distributed shared memory: no workspace, and integers add to the
+// same sum in any order. Rows are written whole, lane = column, so any n, stride and
+// alignment is written in order.
 #pragma once
 
 #include "gemm.cuh"
@@ -33,7 +36,8 @@ struct GemmI8Params {
     int32_t bias_f32;
     int32_t vec_out;         // y rows (tile kernel: and the residual's) take vectors of four values; pairs: TMA stores
     int32_t vec_res;         // pairs: residual rows take TMA loads
-    int32_t x_rows;          // rows of the x box: 128, or fewer when m is small
+    int32_t x_rows;          // tile kernel: rows of the x box: 128, or fewer when m is small
+    int32_t splits;          // tile kernel: CTAs of a tile (the cluster), each with a part of k
     int32_t tail_tiles;      // pair kernel: last-wave tiles cut into `pieces` column pieces
     int32_t pieces;          // 0: none; else 2 or 4
     int* err;
@@ -43,14 +47,15 @@ template <int BN>
 struct GemmI8TileCfg {
     static constexpr int BM = 128;
     static constexpr int BK = 128;  // int8: one swizzle row
-    static constexpr int STAGES = BN == 128 ? 4 : 6;
+    static constexpr int STAGES = BN == 128 ? 6 : 8;
     static constexpr int A_BYTES = BM * BK;
     static constexpr int B_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int THREADS = 192;
+    static constexpr int THREADS = 256;
     static constexpr int ROW = BN + 4;  // int32 words of a staged row: lanes of a warp store to all banks
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 256;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 128 * 4 + 256;
     static_assert(BM * ROW * 4 <= STAGES * STAGE_BYTES, "the staged tile reuses the ring");
+    static_assert((2 * STAGES + 2) * 8 <= 256, "barriers");
 };
 
 // GELU(v) = v Phi(v) = max(v, 0) - a Phi(-a) with a = |v|, and Phi(-a) = 2^Q(a) for a
@@ -123,24 +128,31 @@ __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t 
 }
 
 template <int BN, bool OUT_F32>
-__global__ void __launch_bounds__(192)
+__global__ void __launch_bounds__(256)
     gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                         const GemmI8Params p) {
     using C = GemmI8TileCfg<BN>;
-    extern __shared__ uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+    float* s_xs = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES);  // the tile's x scales
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_xs + 128);
     uint64_t* full_bar = bars;
     uint64_t* empty_bar = bars + C::STAGES;
     uint64_t* done_bar = bars + 2 * C::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
+    const int S = p.splits;
+    const int split = static_cast<int>(blockIdx.x) % S;  // the rank in the cluster
+    const int tile = static_cast<int>(blockIdx.x) / S;
     const int num_n = (p.n + BN - 1) / BN;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.x / num_n) * C::BM;
-    const int n0 = static_cast<int>(blockIdx.x % num_n) * BN;
+    const int64_t m0 = static_cast<int64_t>(tile / num_n) * C::BM;
+    const int n0 = tile % num_n * BN;
     const int num_k = (p.k + C::BK - 1) / C::BK;
+    const int kb_lo = static_cast<int>(static_cast<int64_t>(split) * num_k / S);
+    const int nkb = static_cast<int>(static_cast<int64_t>(split + 1) * num_k / S) - kb_lo;  // >= 1: S <= num_k
+    const int rows = static_cast<int>(p.m - m0 < C::BM ? p.m - m0 : C::BM);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -164,80 +176,60 @@ __global__ void __launch_bounds__(192)
     pdl_wait();
     pdl_launch_dependents();
 
-    bool ok = true;
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         // ------------------------------------------------------------ producer
+        const uint32_t elected = elect_one();
         const uint32_t bytes = static_cast<uint32_t>(p.x_rows * C::BK + C::B_BYTES);
-        int kb = 0;
-        for (; kb < num_k; ++kb) {
-            const int s = kb % C::STAGES;
-            if (!wait_bar(&empty_bar[s], ((kb / C::STAGES) & 1) ^ 1, abort_flag, p.err, 111)) break;
-            uint8_t* sa = smem + s * C::STAGE_BYTES;
-            mbar_arrive_expect_tx(&full_bar[s], bytes);
-            tma_load_2d(sa, &tm_x, &full_bar[s], kb * C::BK, static_cast<int32_t>(m0));
-            tma_load_2d(sa + C::A_BYTES, &tm_w, &full_bar[s], kb * C::BK, n0);
-        }
-        // every load has landed before the ring is used again or the CTA exits
-        for (int i = kb > C::STAGES ? kb - C::STAGES : 0; i < kb; ++i) {
-            volatile int no_abort = 0;
-            wait_bar(&full_bar[i % C::STAGES], (i / C::STAGES) & 1, &no_abort, p.err, 112);
-        }
-    } else if (warp == 1 && lane == 0) {
-        // ------------------------------------------------------------ MMA issuer
-        constexpr uint32_t idesc = umma_idesc_i8(C::BM, BN);
-        for (int kb = 0; kb < num_k; ++kb) {
-            const int s = kb % C::STAGES;
-            if (!wait_bar(&full_bar[s], (kb / C::STAGES) & 1, abort_flag, p.err, 211)) break;
-            tc_fence_after();
-            const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES);
-            const uint64_t a_desc = umma_desc_sw128_kmajor(a_addr);
-            const uint64_t b_desc = umma_desc_sw128_kmajor(a_addr + C::A_BYTES);
-#pragma unroll
-            for (int kk = 0; kk < C::BK / 32; ++kk)
-                umma_i8(tmem_base, a_desc + 2 * kk, b_desc + 2 * kk, idesc, kb + kk != 0);
-            umma_commit(&empty_bar[s]);
-        }
-        umma_commit(done_bar);
-    }
-    __syncwarp();
-    {
-        // the MMAs have read the ring and written TMEM
-        volatile int no_abort = 0;
-        ok = wait_bar(done_bar, 0, &no_abort, p.err, 311);
-        ok = ok && *abort_flag == 0;
-    }
-    tc_fence_after();
-    __syncthreads();
-    // ---------------------------------------------------------------- accumulator to shared memory
-    int32_t* staged = reinterpret_cast<int32_t*>(smem);
-    const int rows = static_cast<int>(p.m - m0 < C::BM ? p.m - m0 : C::BM);
-    if (warp >= 2) {
-        const int q = warp & 3;  // TMEM lane quarter of this warp
-        const int r = 32 * q + lane;
-        if (32 * q < rows) {
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(32 * q) << 16) + c, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int g = 0; g < 8; ++g)
-                    *reinterpret_cast<uint4*>(staged + r * C::ROW + c + 4 * g) =
-                        make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        const uint32_t ring = smem_u32(smem), full0 = smem_u32(full_bar);
+        int stage = 0;
+        uint32_t phase = 0;
+        int i = 0;
+        for (; i < nkb; ++i) {
+            if (!__all_sync(0xffffffffu, wait_bar(&empty_bar[stage], phase ^ 1, abort_flag, p.err, 111))) break;
+            const uint32_t sa = ring + stage * C::STAGE_BYTES;
+            mbar_arrive_expect_tx_elected(elected, full0 + 8 * stage, bytes);
+            tma_load_2d_elected(elected, sa, &tm_x, full0 + 8 * stage, (kb_lo + i) * C::BK, static_cast<int32_t>(m0));
+            tma_load_2d_elected(elected, sa + C::A_BYTES, &tm_w, full0 + 8 * stage, (kb_lo + i) * C::BK, n0);
+            if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
             }
         }
-        tc_fence_before();
+        // every load has landed before the ring is used again or the CTA exits
+        for (int b = i > C::STAGES ? i - C::STAGES : 0; b < i; ++b) {
+            volatile int no_abort = 0;
+            wait_bar(&full_bar[b % C::STAGES], (b / C::STAGES) & 1, &no_abort, p.err, 112);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        const uint32_t elected = elect_one();
+        constexpr uint32_t idesc = umma_idesc_i8(C::BM, BN);
+        const uint64_t a_desc0 = umma_desc_sw128_kmajor(smem_u32(smem));
+        const uint64_t b_desc0 = umma_desc_sw128_kmajor(smem_u32(smem) + C::A_BYTES);
+        const uint32_t empty0 = smem_u32(empty_bar);
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < nkb; ++i) {
+            if (!__all_sync(0xffffffffu, wait_bar(&full_bar[stage], phase, abort_flag, p.err, 211))) break;
+            tc_fence_after();
+            const uint64_t at = static_cast<uint64_t>(stage * (C::STAGE_BYTES >> 4));
+#pragma unroll
+            for (int kk = 0; kk < C::BK / 32; ++kk)
+                umma_i8_elected(elected, tmem_base, a_desc0 + at + 2 * kk, b_desc0 + at + 2 * kk, idesc, i + kk != 0);
+            umma_commit_elected(elected, empty0 + 8 * stage);
+            if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        umma_commit_elected(elected, smem_u32(done_bar));
     }
-    __syncthreads();
-    tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem_base, BN);
-    if (!ok) return;
-    // ---------------------------------------------------------------- scales, bias, activation, residual
-    constexpr int LANES = BN / 4;           // threads of a row, four columns each
+    // what the outputs need besides the sums is on its way meanwhile
+    constexpr int LANES = BN / 4;             // threads of a row, four columns each
     constexpr int STEP = C::THREADS / LANES;  // rows at once
-    const int col = n0 + 4 * (threadIdx.x % LANES);
+    const int my = threadIdx.x % LANES;
+    const int col = n0 + 4 * my;
     const int live = p.n - col < 4 ? p.n - col : 4;
-    if (live <= 0) return;
     float ws[4], b[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -247,13 +239,75 @@ __global__ void __launch_bounds__(192)
             b[e] = p.bias_f32 ? static_cast<const float*>(p.bias)[col + e]
                               : __half2float(static_cast<const __half*>(p.bias)[col + e]);
     }
-    for (int r = threadIdx.x / LANES; r < rows; r += STEP) {
-        const float xs = __ldg(p.x_scale + m0 + r);
-        const int4 a = *reinterpret_cast<const int4*>(staged + r * C::ROW + 4 * (threadIdx.x % LANES));
-        float v[4] = {fmaf(__int2float_rn(a.x) * ws[0], xs, b[0]), fmaf(__int2float_rn(a.y) * ws[1], xs, b[1]),
-                      fmaf(__int2float_rn(a.z) * ws[2], xs, b[2]), fmaf(__int2float_rn(a.w) * ws[3], xs, b[3])};
-        store_i8_outputs<OUT_F32>(p, m0 + r, col, live, v);
+    if (threadIdx.x < 128) s_xs[threadIdx.x] = static_cast<int>(threadIdx.x) < rows ? __ldg(p.x_scale + m0 + threadIdx.x) : 0.0f;
+    __syncwarp();
+    volatile int no_abort = 0;
+    bool ok = wait_bar(done_bar, 0, &no_abort, p.err, 311);  // the MMAs have read the ring and written TMEM
+    ok = ok && *abort_flag == 0;
+    tc_fence_after();
+    __syncthreads();
+    // ---------------------------------------------------------------- sums to shared memory
+    int32_t* staged = reinterpret_cast<int32_t*>(smem);
+    {
+        const int q = warp & 3;  // TMEM lane quarter of this warp
+        const int r = 32 * q + lane;
+        constexpr int HALF = BN / 2;
+        if (32 * q < rows) {
+#pragma unroll
+            for (int c = (warp >> 2) * HALF; c < (warp >> 2) * HALF + HALF; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(32 * q) << 16) + c, v);
+                tmem_ld_wait(v);
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                    *reinterpret_cast<uint4*>(staged + r * C::ROW + c + 4 * g) =
+                        make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+            }
+        }
+        tc_fence_before();
     }
+    if (S > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem_base, BN);
+    // ---------------------------------------------------------------- scales, bias, activation, residual
+    const int r_lo = split * rows / S, r_hi = (split + 1) * rows / S;
+    if (ok && live > 0) {
+        for (int r0 = r_lo + threadIdx.x / LANES; r0 < r_hi; r0 += 4 * STEP) {
+            int4 a[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + i * STEP;
+                if (r < r_hi) a[i] = *reinterpret_cast<const int4*>(staged + r * C::ROW + 4 * my);
+            }
+            if (S > 1) {
+                for (int o = 1; o < S; ++o) {
+                    const uint32_t from = static_cast<uint32_t>(split + o < S ? split + o : split + o - S);
+                    const uint32_t base = mapa_shared(smem_u32(staged + 4 * my), from);
+                    int4 t[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (r0 + i * STEP < r_hi) t[i] = ld_shared_cluster_v4(base + (r0 + i * STEP) * C::ROW * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (r0 + i * STEP < r_hi) a[i].x += t[i].x, a[i].y += t[i].y, a[i].z += t[i].z, a[i].w += t[i].w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + i * STEP;
+                if (r >= r_hi) break;
+                const float xs = s_xs[r];
+                float v[4] = {fmaf(__int2float_rn(a[i].x) * ws[0], xs, b[0]), fmaf(__int2float_rn(a[i].y) * ws[1], xs, b[1]),
+                              fmaf(__int2float_rn(a[i].z) * ws[2], xs, b[2]), fmaf(__int2float_rn(a[i].w) * ws[3], xs, b[3])};
+                store_i8_outputs<OUT_F32>(p, m0 + r, col, live, v);
+            }
+        }
+    }
+    __syncwarp();
+    if (S > 1) cluster_sync();  // no CTA leaves while another reads its sums
 }
 
 }  // namespace rpfq

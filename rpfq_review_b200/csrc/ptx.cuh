@@ -114,6 +114,16 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
     return r;
 }
 
+// 16 bytes of shared memory of any CTA of the cluster (shared::cluster address).
+__device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 // All threads of all CTAs of the cluster (release / acquire).
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -358,6 +368,17 @@ __device__ __forceinline__ void tma_load_2d_pair_elected(uint32_t elected, uint3
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_2d_elected(uint32_t elected, uint32_t dst, const CUtensorMap* m, uint32_t bar,
+                                                    int32_t c0, int32_t c1) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(elected)
+        : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx_elected(uint32_t elected, uint32_t bar, uint32_t bytes) {
     asm volatile(
         "{\n\t.reg .pred e;\n\t"
@@ -367,7 +388,19 @@ __device__ __forceinline__ void mbar_arrive_expect_tx_elected(uint32_t elected, 
         : "memory");
 }
 
-// umma_i8_pair by the elected lane.
+// D[tmem] (+)= A[smem] * B[smem]^T, int8 inputs, int32 accumulate (kind::i8, K = 32
+// per instruction), for one CTA and for a CTA pair (M = 256).
+__device__ __forceinline__ void umma_i8_elected(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+
 __device__ __forceinline__ void umma_i8_pair_elected(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                                      uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -379,6 +412,16 @@ __device__ __forceinline__ void umma_i8_pair_elected(uint32_t elected, uint32_t 
         : "memory");
 }
 
+// Arrive on this CTA's barrier when the MMAs issued so far have completed.
+__device__ __forceinline__ void umma_commit_elected(uint32_t elected, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
+}
+
 // Arrive on the barrier at this shared-memory offset in both CTAs of the pair when
 // the pair MMAs issued so far have completed; by the elected lane.
 __device__ __forceinline__ void umma_commit_both_elected(uint32_t elected, uint32_t bar) {
@@ -387,28 +430,6 @@ __device__ __forceinline__ void umma_commit_both_elected(uint32_t elected, uint3
         "setp.ne.b32 e, %2, 0;\n\t"
         "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
         "h"(static_cast<uint16_t>(3)), "r"(elected)
-        : "memory");
-}
-
-// D[tmem] (+)= A[smem] * B[smem]^T, int8 inputs, int32 accumulate (kind::i8,
-// K = 32 per instruction), for one CTA and for a CTA pair.
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 

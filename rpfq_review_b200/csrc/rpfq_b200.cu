@@ -841,9 +841,9 @@ int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t 
     if (!rc) rc = make_tmap_i8(&tw, a->w, a->n, a->k, a->ldw, BN);
     if (rc) return rc;
     const int64_t tiles = ((a->m + 127) / 128) * ((a->n + BN - 1) / BN);
-    if (tiles > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
-    RPFQ_CUDA(launch_kernel(gemm_i8_tile_kernel<BN, OUT_F32>, dim3(static_cast<unsigned>(tiles)), dim3(C::THREADS),
-                            C::SMEM_BYTES, stream, 1, tx, tw, p));
+    if (tiles * p.splits > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
+    RPFQ_CUDA(launch_kernel(gemm_i8_tile_kernel<BN, OUT_F32>, dim3(static_cast<unsigned>(tiles * p.splits)),
+                            dim3(C::THREADS), C::SMEM_BYTES, stream, p.splits, tx, tw, p));
     return RPFQ_OK;
 }
 
@@ -948,6 +948,96 @@ int launch_i8_few_rows(const GemmI8FewParams& p, cudaStream_t stream) {
     return launch_i8_few<kFewRows, 4, XT, OUT_F32>(p, stream);
 }
 
+// Clusters of `splits` tile-kernel CTAs that fit on the device at once (one CTA per
+// SM; queried once per device and size).
+template <int BN>
+int i8_max_clusters(int splits, DeviceState* st) {
+    if (splits == 1) return st->sm_count;
+    static std::once_flag once[kMaxDevices][kMaxSplits + 1];
+    static int fit[kMaxDevices][kMaxSplits + 1] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+    std::call_once(once[dev][splits], [dev, splits, st]() {
+        using C = GemmI8TileCfg<BN>;
+        if (cudaFuncSetAttribute(gemm_i8_tile_kernel<BN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::SMEM_BYTES) != cudaSuccess) {
+            cudaGetLastError();
+            return;
+        }
+        cudaLaunchConfig_t q = {};
+        cudaLaunchAttribute qa[1];
+        qa[0].id = cudaLaunchAttributeClusterDimension;
+        qa[0].val.clusterDim.x = splits;
+        qa[0].val.clusterDim.y = 1;
+        qa[0].val.clusterDim.z = 1;
+        q.gridDim = dim3(st->sm_count / splits * splits);
+        q.blockDim = dim3(C::THREADS);
+        q.dynamicSmemBytes = C::SMEM_BYTES;
+        q.attrs = qa;
+        q.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_tile_kernel<BN, false>, &q) != cudaSuccess) {
+            cudaGetLastError();
+            return;
+        }
+        fit[dev][splits] = n;
+    });
+    return fit[dev][splits];
+}
+
+struct I8Plan {
+    int bn;      // 64 or 128: tile kernel; 256: CTA pairs
+    int splits;  // k parts per tile (tile kernel)
+};
+
+// Tile width and k parts of one call, by the least estimated time (us, fitted to
+// CUDA-graph timings on B200 over m = 16..4000, n = 300..4096, k = 390..4096; kb:
+// k-blocks of 128). A wave of the tile kernel costs 2.3, 0.010 (64 columns) or 0.021
+// (128) per live row of its epilogue and 0.15 per k-block of a CTA (an SM streams the
+// operands alone); a split adds 0.7 + 0.0016 rows S for the cluster's exchange. CTA pairs
+// start at 3.9 + 0.28 kb, and a further wave costs max(0.28 kb, 2) + 0.3, its tiles cut
+// when it is at most half full. Measured (us, 64 / 128 wide, best S / pairs): 197 x
+// 1024 x 1024 (m, n, k) 4.6 / 5.8 / 6.1; 64 x 1024 x 4096 4.9 / 5.5 / 12.2; 1576 x 1024
+// x 4096 16.3 / 10.5 / 12.9; 1576 x 768 x 768 8.0 / 5.8 / 5.7; 3152 x 768 x 768 12.8 /
+// 10.0 / 6.1. More than four parts were never the best.
+I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
+    const int kb = (a->k + 127) / 128;
+    if (a->block_n == 256) return {256, 1};
+    const int forced = a->split_k ? std::min(a->split_k, kb) : 0;
+    const double rows = static_cast<double>(std::min<int64_t>(a->m, 128));
+    const int64_t row_tiles = (a->m + 127) / 128;
+    I8Plan best = {a->block_n ? a->block_n : 128, forced ? forced : 1};
+    double cost = -1.0;
+    for (int bn : {64, 128}) {
+        if (a->block_n && bn != a->block_n) continue;
+        for (int s : {1, 2, 4}) {
+            if (forced) s = forced;
+            if (s > kb) break;
+            const int fit = bn == 64 ? i8_max_clusters<64>(s, st) : i8_max_clusters<128>(s, st);
+            if (fit <= 0) continue;
+            const int64_t tiles = row_tiles * ((a->n + bn - 1) / bn);
+            const double waves = static_cast<double>((tiles + fit - 1) / fit);
+            const double c = waves * (2.3 + (bn == 64 ? 0.010 : 0.021) * rows + 0.15 * ((kb + s - 1) / s)) +
+                             (s > 1 ? 0.7 + 0.0016 * rows * s : 0.0);
+            if (cost < 0 || c < cost) {
+                cost = c;
+                best = {bn, s};
+            }
+            if (forced) break;
+        }
+    }
+    if (a->block_n || a->split_k > 1) return best;
+    const int64_t pair_tiles = ((a->m + 255) / 256) * ((a->n + 255) / 256);
+    const int units = std::max(1, st->sm_count / 2);
+    const int64_t rest = pair_tiles % units;
+    const double more = pair_tiles <= units ? 0.0
+                                            : static_cast<double>(pair_tiles / units - 1) +
+                                                  (rest == 0 ? 0.0 : (2 * rest <= units ? 0.5 : 1.0));
+    const double pairs = 3.9 + 0.28 * kb + more * (std::max(0.28 * kb, 2.0) + 0.3);
+    if (cost < 0 || pairs < cost) best = {256, 1};
+    return best;
+}
+
 int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     const char* who = "rpfq_gemm_i8_sm100";
     if (!args) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
@@ -983,8 +1073,13 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
     if (a->residual && (((a->flags & RPFQ_GEMM_RESIDUAL_F32) != 0) != ((a->flags & RPFQ_GEMM_OUT_F32) != 0)))
         return fail(RPFQ_ERR_UNSUPPORTED, "%s: the residual must have the output's dtype", who);
-    const bool few = few_rows_fit(a->m, a->k);
-    const uint64_t need = x_flags ? rpfq_gemm_i8_scratch_bytes(a->m, a->k) : 0;
+    if (a->block_n != 0 && a->block_n != 64 && a->block_n != 128 && a->block_n != 256)
+        return fail(RPFQ_ERR_INVALID, "%s: block_n must be 0, 64, 128 or 256 (got %d)", who, a->block_n);
+    if (a->split_k < 0 || a->split_k > kMaxSplits || (a->split_k > 1 && a->block_n == 256))
+        return fail(RPFQ_ERR_INVALID, "%s: split_k must be 0..%d, and at most 1 with block_n 256 (got %d)", who, kMaxSplits,
+                    a->split_k);
+    const bool few = a->block_n == 0 && a->split_k == 0 && few_rows_fit(a->m, a->k);
+    const uint64_t need = x_flags && !few ? static_cast<uint64_t>(a->m) * ((a->k + 15) / 16 * 16 + 4) : 0;
     if (need && (!a->scratch || !aligned16(a->scratch) || a->scratch_bytes < need))
         return fail(RPFQ_ERR_INVALID, "%s: quantizing %lld rows needs 16-byte aligned scratch of %llu bytes", who,
                     (long long)a->m, (unsigned long long)need);
@@ -1017,6 +1112,7 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     p.bias_f32 = (a->flags & RPFQ_GEMM_BIAS_F32) ? 1 : 0;
     p.vec_out = i8_vec_out(a) ? 1 : 0;
     p.x_rows = a->m >= 128 ? 128 : static_cast<int32_t>((a->m + 7) / 8 * 8);
+    p.splits = 1;
     p.vec_res = p.tail_tiles = p.pieces = 0;
     p.err = st->err_word;
     const bool f32 = (a->flags & RPFQ_GEMM_OUT_F32) != 0;
@@ -1035,15 +1131,16 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
             return f32 ? launch_i8_few_rows<kXFloat, true>(fp, stream) : launch_i8_few_rows<kXFloat, false>(fp, stream);
         return f32 ? launch_i8_few_rows<kXCodes, true>(fp, stream) : launch_i8_few_rows<kXCodes, false>(fp, stream);
     }
-    const int64_t pair_tiles = ((a->m + 255) / 256) * ((a->n + 255) / 256);
-    if (pair_tiles >= st->sm_count / 2) {
+    const I8Plan plan = plan_i8(a, st);
+    if (plan.bn == 256) {
         if (res) return f32 ? launch_i8_pair<true, true, 8>(a, p, st, stream) : launch_i8_pair<false, true, 8>(a, p, st, stream);
         if (p.activation == RPFQ_ACT_GELU)
             return f32 ? launch_i8_pair<true, false, 16>(a, p, st, stream) : launch_i8_pair<false, false, 16>(a, p, st, stream);
         return f32 ? launch_i8_pair<true, false, 8>(a, p, st, stream) : launch_i8_pair<false, false, 8>(a, p, st, stream);
     }
-    return (a->flags & RPFQ_GEMM_OUT_F32) ? launch_i8_tile<128, true>(a, p, stream)
-                                          : launch_i8_tile<128, false>(a, p, stream);
+    p.splits = plan.splits;
+    if (plan.bn == 64) return f32 ? launch_i8_tile<64, true>(a, p, stream) : launch_i8_tile<64, false>(a, p, stream);
+    return f32 ? launch_i8_tile<128, true>(a, p, stream) : launch_i8_tile<128, false>(a, p, stream);
 }
 
 // ---------------------------------------------------------------- rotary positions

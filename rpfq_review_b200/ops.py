@@ -585,13 +585,13 @@ def quantize_rows(x: torch.Tensor):
 
 
 def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x_scale, x_flag: int, w: torch.Tensor,
-               w_scale: torch.Tensor, bias, residual, activation, out, out_dtype) -> torch.Tensor:
+               w_scale: torch.Tensor, bias, residual, activation, out, out_dtype, block_n, split_k) -> torch.Tensor:
     """What gemm_int8 and linear_int8 share: the checks of everything but x, and the launch."""
     index = x.get_device()
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _gemm_int8(name, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
-                              out_dtype)
+                              out_dtype, block_n, split_k)
     n, k = w.shape
     _require(w_scale, "w_scale", torch.float32)
     if w_scale.numel() != n:
@@ -625,12 +625,12 @@ def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x
     L = _lib.lib()
     scratch, need = None, 0
     if x_flag:
-        need = L.rpfq_gemm_i8_scratch_bytes(m, k)
+        need = m * ((k + 15) // 16 * 16 + 4) if block_n or split_k else L.rpfq_gemm_i8_scratch_bytes(m, k)
         if need:
             scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
     a = _lib.RpfqGemmI8Args(x2.data_ptr(), ldx, x_scale, w2.data_ptr(), ldw, w_scale.data_ptr(), bias_ptr, r_ptr, ldr,
                             out.data_ptr(), ldy, m, n, k, _ACT[activation], x_flag | _flags(out, r2, bias),
-                            _p(scratch), need)
+                            block_n, split_k, _p(scratch), need)
     _lib.check(L.rpfq_gemm_i8_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index)), "rpfq_gemm_i8_sm100")
     if m:
         _count_launch(2 if need else 1)
@@ -645,14 +645,17 @@ def _check_codes(name: str, w: torch.Tensor) -> None:
 
 def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
               bias: torch.Tensor | None = None, residual: torch.Tensor | None = None, activation="none",
-              out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+              out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16, block_n: int = 0,
+              split_k: int = 0) -> torch.Tensor:
     """``act(x_scale[..., None] * w_scale * (x @ w.T) + bias) + residual`` of
     int8 codes ``x[..., k]`` and ``w[n, k]`` with a scale per token and per output
     channel (``rpfq_gemm_i8_sm100``): exact int32 sums on the tensor cores
     (k up to ``GEMM_INT8_MAX_K``), scaled in fp32. ``bias`` fp16 or fp32;
     ``residual`` and ``out`` fp16 or fp32 alike (and may be the same tensor for
     an in-place residual add). Code rows that do not start on 16 bytes are
-    copied into rows that do; :func:`quantize_rows` returns such rows."""
+    copied into rows that do; :func:`quantize_rows` returns such rows.
+    ``block_n`` (64, 128, 256) and ``split_k`` (1..8) fix the tiles and the parts
+    of k, 0 leaves them to the library; the result is the same bit for bit."""
     name = "gemm_int8"
     _require(x, "x", torch.int8)
     _check_codes(name, w)
@@ -664,12 +667,12 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     _same_device(name, x.get_device(), x_scale=x_scale)
     x_scale = x_scale.contiguous()
     return _gemm_int8(name, x, x2, m, ldx, x_scale.data_ptr(), 0, w, w_scale, bias, residual, activation, out,
-                      out_dtype)
+                      out_dtype, block_n, split_k)
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 residual: torch.Tensor | None = None, activation="none", out: torch.Tensor | None = None,
-                out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+                out_dtype: torch.dtype = torch.float16, block_n: int = 0, split_k: int = 0) -> torch.Tensor:
     """The 8-bit linear layer of fp16 or fp32 activations ``x[..., k]``: the rows
     of x as :func:`quantize_rows` codes them, then :func:`gemm_int8` with the
     weight's codes and scales (``w, w_scale = quantize_rows(weight)``), the same
@@ -679,7 +682,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     _check_codes(name, w)
     _forward_only(name, x, w_scale, residual)
     x2, m, ldx = _matrix(x, w.shape[1], "x")
-    return _gemm_int8(name, x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out, out_dtype)
+    return _gemm_int8(name, x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out, out_dtype,
+                      block_n, split_k)
 
 
 # ---------------------------------------------------------------------------

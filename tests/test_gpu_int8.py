@@ -330,3 +330,28 @@ def test_few_rows_same_bits(cuda, m, n, k):
             odd = torch.zeros(m, k + 3, dtype=src.dtype, device=cuda)[:, 1:1 + k]
             odd.copy_(src[3:3 + m])
             assert torch.equal(ops.linear_int8(odd, w, ws, bias, res[3:3 + m], "gelu", out_dtype=dtype), few)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 128), (3, 130, 1025), (9, 1000, 2048), (130, 200, 257), (200, 64, 4000), (300, 333, 900)])
+def test_gemm_int8_tiles_and_splits_same_bits(cuda, m, n, k):
+    """Every tile width and number of k parts (more parts than k-blocks included) gives
+    the same bits: the sums are exact."""
+    from rpfq_review_b200 import _lib, ops
+    g = torch.Generator().manual_seed(m + n + k)
+    x = torch.randn(m, k, generator=g).to(cuda)
+    xq, xs = ops.quantize_rows(x)
+    w, ws = ops.quantize_rows((torch.randn(n, k, generator=g) * 0.1).to(cuda))
+    bias = torch.randn(n, generator=g).to(cuda)
+    for dtype in (torch.float16, torch.float32):
+        res = torch.randn(m, n, generator=g).to(dtype).to(cuda)
+        want = ops.gemm_int8(xq, xs, w, ws, bias, res, "gelu", out_dtype=dtype)
+        _check(want, _product_ref(xq, xs, w, ws, bias, "gelu", res, dtype))
+        for bn, splits in [(b, s) for b in (64, 128) for s in range(1, 9)] + [(256, 0), (256, 1), (0, 3)]:
+            y = ops.gemm_int8(xq, xs, w, ws, bias, res, "gelu", out_dtype=dtype, block_n=bn, split_k=splits)
+            assert torch.equal(y, want), (bn, splits)
+        assert torch.equal(ops.linear_int8(x, w, ws, bias, res, "gelu", out_dtype=dtype, block_n=64, split_k=2), want)
+        inplace = res.clone()
+        ops.gemm_int8(xq, xs, w, ws, bias, inplace, "gelu", out=inplace, split_k=4)
+        assert torch.equal(inplace, want)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0

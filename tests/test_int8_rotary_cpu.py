@@ -16,7 +16,7 @@ A = 4096  # a 16-byte aligned address; nothing is read
 
 
 def test_struct_sizes():
-    assert ctypes.sizeof(_lib.RpfqGemmI8Args) == 8 * 12 + 4 * 4 + 8 * 2
+    assert ctypes.sizeof(_lib.RpfqGemmI8Args) == 8 * 12 + 4 * 6 + 8 * 2
     assert ctypes.sizeof(_lib.RpfqRotaryArgs) == 8 * 13 + 4 * 10
 
 
@@ -33,6 +33,7 @@ def _gemm(**kw):
     dict(ldy=31), dict(residual=A, ldr=31), dict(y=A + 1), dict(y=A + 2, flags=1), dict(bias=A + 1),
     dict(bias=A + 2, flags=4), dict(residual=A + 1, ldr=32), dict(x_scale=A + 2), dict(w_scale=A + 1),
     dict(flags=32), dict(flags=24), dict(activation=2), dict(activation=-1),
+    dict(block_n=96), dict(block_n=-1), dict(split_k=9), dict(split_k=-1), dict(block_n=256, split_k=2),
     dict(flags=8, x=A + 1), dict(flags=16, x=A + 2), dict(flags=8, ldx=59), dict(flags=8, m=9),
     dict(flags=8, m=9, scratch=A + 4, scratch_bytes=1 << 20), dict(flags=8, m=9, scratch=A, scratch_bytes=9 * 68 - 1)])
 def test_gemm_i8_rejects(bad):

@@ -184,8 +184,8 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
  * residual has y's dtype. Nothing is kept between calls.
  * With RPFQ_GEMM_X_F16 or RPFQ_GEMM_X_F32 in flags, x holds fp16 or fp32
  * activations (any row stride >= k, x_scale unused): their rows are quantized
- * as by rpfq_quantize_rows_sm100, inside the product's launch for at most 8
- * rows and into `scratch` otherwise. scratch is device memory, 16-byte
+ * as by rpfq_quantize_rows_sm100, inside the product's launch for a few rows
+ * and into `scratch` otherwise. scratch is device memory, 16-byte
  * aligned, of at least rpfq_gemm_i8_scratch_bytes(m, k) bytes (NULL where that
  * is 0; with block_n or split_k given, m * (round_up(k, 16) + 4)); calls that
  * may overlap on the GPU need their own. The result is that of the two calls,

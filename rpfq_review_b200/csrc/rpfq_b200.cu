@@ -919,8 +919,14 @@ bool i8_vec_out(const RpfqGemmI8Args* a) {
     return !a->residual || (reinterpret_cast<uintptr_t>(a->residual) % bytes == 0 && a->ldr % 4 == 0);
 }
 
-// Rows that the few-row kernel takes: their codes lie in its shared memory.
-bool few_rows_fit(int64_t m, int64_t k) { return m <= kFewRows && m * ((k + 15) / 16 * 16) <= kFewSmem; }
+// Rows that the few-row kernel takes; their codes lie in its shared memory. Up to
+// four it is ahead of the tensor-core tiles (us, few / tiles at n x k: 1 row 1024 x
+// 4096 2.3 / 4.6; 4 rows 768 x 768 2.3 / 3.1, 4096 x 4096 6.0 / 5.7); with rows to
+// quantize the tiles need a launch more, which up to eight rows of at most 2048
+// values repays (8 rows 768 x 768 3.6 / 5.3, 1024 x 4096 10.5 / 7.1).
+bool few_rows_fit(int64_t m, int64_t k, bool quantize) {
+    return (m <= 4 || (quantize && m <= kFewRows && k <= 2048)) && m * ((k + 15) / 16 * 16) <= kFewSmem;
+}
 
 template <int ROWS, int COLS, int XT, bool OUT_F32>
 int launch_i8_few(const GemmI8FewParams& p, cudaStream_t stream) {
@@ -944,8 +950,10 @@ template <int XT, bool OUT_F32>
 int launch_i8_few_rows(const GemmI8FewParams& p, cudaStream_t stream) {
     if (p.g.m == 1) return launch_i8_few<1, 1, XT, OUT_F32>(p, stream);
     if (p.g.m == 2) return launch_i8_few<2, 2, XT, OUT_F32>(p, stream);
-    if (p.g.m <= 4) return launch_i8_few<4, 2, XT, OUT_F32>(p, stream);
-    return launch_i8_few<kFewRows, 4, XT, OUT_F32>(p, stream);
+    if constexpr (XT != kXCodes) {
+        if (p.g.m > 4) return launch_i8_few<kFewRows, 4, XT, OUT_F32>(p, stream);
+    }
+    return launch_i8_few<4, 2, XT, OUT_F32>(p, stream);
 }
 
 // Clusters of `splits` tile-kernel CTAs that fit on the device at once (one CTA per
@@ -1078,7 +1086,7 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     if (a->split_k < 0 || a->split_k > kMaxSplits || (a->split_k > 1 && a->block_n == 256))
         return fail(RPFQ_ERR_INVALID, "%s: split_k must be 0..%d, and at most 1 with block_n 256 (got %d)", who, kMaxSplits,
                     a->split_k);
-    const bool few = a->block_n == 0 && a->split_k == 0 && few_rows_fit(a->m, a->k);
+    const bool few = a->block_n == 0 && a->split_k == 0 && few_rows_fit(a->m, a->k, x_flags != 0);
     const uint64_t need = x_flags && !few ? static_cast<uint64_t>(a->m) * ((a->k + 15) / 16 * 16 + 4) : 0;
     if (need && (!a->scratch || !aligned16(a->scratch) || a->scratch_bytes < need))
         return fail(RPFQ_ERR_INVALID, "%s: quantizing %lld rows needs 16-byte aligned scratch of %llu bytes", who,
@@ -1330,7 +1338,7 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
 }
 
 uint64_t rpfq_gemm_i8_scratch_bytes(int64_t m, int32_t k) {
-    if (m <= 0 || k <= 0 || few_rows_fit(m, k)) return 0;
+    if (m <= 0 || k <= 0 || few_rows_fit(m, k, true)) return 0;
     return static_cast<uint64_t>(m) * ((k + 15) / 16 * 16 + 4);
 }
 

@@ -310,7 +310,8 @@ def test_packed_layer_int8(cuda, n_c, k_c):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 5, 1), (1, 1000, 768), (2, 33, 17), (3, 4097, 100), (4, 64, 4096), (5, 31, 257),
-                                   (7, 1000, 1003), (8, 770, 2048), (8, 9, 12288), (8, 20, 12304), (1, 7, 98304), (1, 7, 98320)])
+                                   (7, 1000, 1003), (8, 770, 2048), (8, 9, 12288), (8, 20, 12304), (4, 5, 24576),
+                                   (4, 6, 24592), (1, 7, 98304), (1, 7, 98320)])
 def test_few_rows_same_bits(cuda, m, n, k):
     """Few rows run on their own kernel (and quantize inside it); rows of a larger
     product on the tensor cores: the same bits, for codes, fp16 and fp32."""

@@ -1152,11 +1152,42 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- rotary positions
+// Threads of a token and tokens of a block: 32 threads a token (16 to 32 are alike, 64
+// cost 10 % on 32 heads of 64: fewer heads per thread to run ahead over), 16 tokens a
+// block while four blocks an SM remain (8 are alike, 32 and 64 cost 5 % and more in
+// the last wave). With fewer tokens than that, more threads a token and fewer
+// tokens a block.
+template <typename T, int BYTES, bool INTERLEAVED>
+cudaError_t launch_rotary_one(RotaryParams p, DeviceState* st, cudaStream_t stream) {
+    const int pieces = RotaryPieces<T, BYTES, INTERLEAVED>::all(p.dim, p.pairs, p.copy_rest != 0);
+    const int span = std::min(pieces, kRotaryThreads);
+    auto steps = [&](int threads) { return std::max(1, std::min(p.heads, threads / span)); };
+    const int64_t blocks_wanted = int64_t(4) * st->sm_count;
+    p.head_step = steps(32);
+    int slots = kRotaryThreads / (span * p.head_step);
+    while (slots > 1 && (p.tokens + slots - 1) / slots < blocks_wanted) {
+        const int more = steps(2 * span * p.head_step);
+        if (more == p.head_step) break;
+        p.head_step = more;
+        slots = kRotaryThreads / (span * p.head_step);
+    }
+    const int most = std::max(1, std::min(kRotaryTokens, kRotaryTable / p.pairs));
+    int tile = std::min(slots, most);
+    while (2 * tile <= std::min(most, 16) && p.tokens / (2 * tile) >= blocks_wanted) tile *= 2;
+    p.token_tile = tile;
+    const int64_t blocks = (p.tokens + tile - 1) / tile;
+    // at most 32 KB of copies and 16 KB of cos / sin: below the 48 KB that need no opt-in
+    const size_t smem = static_cast<size_t>(kRotaryDepth) * 2 * kRotaryThreads * BYTES +
+                        static_cast<size_t>(tile) * p.pairs * sizeof(float2);
+    return launch_kernel(rotary_kernel<T, BYTES, INTERLEAVED>, dim3(static_cast<unsigned>(blocks)), dim3(kRotaryThreads),
+                         smem, stream, 1, p);
+}
+
 template <typename T, bool INTERLEAVED>
-cudaError_t launch_rotary(int bytes, dim3 grid, cudaStream_t stream, const RotaryParams& p) {
-    if (bytes == 16) return launch_kernel(rotary_kernel<T, 16, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
-    if (bytes == 8) return launch_kernel(rotary_kernel<T, 8, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
-    return launch_kernel(rotary_kernel<T, 0, INTERLEAVED>, grid, dim3(kRotaryThreads), 0, stream, 1, p);
+cudaError_t launch_rotary(int bytes, DeviceState* st, cudaStream_t stream, const RotaryParams& p) {
+    if (bytes == 16) return launch_rotary_one<T, 16, INTERLEAVED>(p, st, stream);
+    if (bytes == 8) return launch_rotary_one<T, 8, INTERLEAVED>(p, st, stream);
+    return launch_rotary_one<T, 0, INTERLEAVED>(p, st, stream);
 }
 
 // Whether rows and runs of this call can move in vectors of `bytes`.
@@ -1351,6 +1382,7 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     if (!a) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
     if (a->batch < 0 || a->length < 0 || a->heads < 0 || a->dim <= 0)
         return fail(RPFQ_ERR_INVALID, "%s: bad shape", who);
+    if (a->heads > (1 << 24)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: at most %d heads", who, 1 << 24);
     if (a->pairs <= 0 || a->pairs > a->dim / 2)
         return fail(RPFQ_ERR_INVALID, "%s: 2 * pairs must be in 2..dim (pairs=%d dim=%d)", who, a->pairs, a->dim);
     if (a->pairs > kRotaryTable) return fail(RPFQ_ERR_UNSUPPORTED, "%s: at most %d pairs", who, kRotaryTable);
@@ -1360,7 +1392,6 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
         return fail(RPFQ_ERR_INVALID, "%s: unknown position type %d", who, a->position_type);
     if (a->batch == 0 || a->length == 0 || a->heads == 0) return RPFQ_OK;
     if (!a->x || !a->y || !a->positions || !a->inv_freq) return fail(RPFQ_ERR_INVALID, "%s: null pointer", who);
-    if (a->heads > 65535) return fail(RPFQ_ERR_UNSUPPORTED, "%s: at most 65535 heads", who);
     const int esize = a->f32 ? 4 : 2;
     const int psize = (a->position_type == RPFQ_POS_I32 || a->position_type == RPFQ_POS_F32) ? 4 : 8;
     if (reinterpret_cast<uintptr_t>(a->x) % esize || reinterpret_cast<uintptr_t>(a->y) % esize ||
@@ -1391,17 +1422,13 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     p.copy_rest = copy_rest ? 1 : 0;
     p.magnitude = a->magnitude;
     p.sign = a->transpose ? -1.0f : 1.0f;
-    p.token_tile = std::max(1, std::min(32, kRotaryTable / a->pairs));
-    p.head_tile = a->heads;
-    const int64_t blocks = (p.tokens + p.token_tile - 1) / p.token_tile;
-    if (blocks > 0x7fffffff || a->length > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: too many tokens", who);
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((p.heads + p.head_tile - 1) / p.head_tile));
+    if (p.tokens > 0x7fffffff || a->length > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: too many tokens", who);
     const int bytes = rotary_vec(a, esize, 16, copy_rest) ? 16 : (rotary_vec(a, esize, 8, copy_rest) ? 8 : 0);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    RPFQ_CUDA((a->f32 ? (a->interleaved ? launch_rotary<float, true>(bytes, grid, cs, p)
-                                        : launch_rotary<float, false>(bytes, grid, cs, p))
-                      : (a->interleaved ? launch_rotary<__half, true>(bytes, grid, cs, p)
-                                        : launch_rotary<__half, false>(bytes, grid, cs, p))));
+    RPFQ_CUDA((a->f32 ? (a->interleaved ? launch_rotary<float, true>(bytes, st, cs, p)
+                                        : launch_rotary<float, false>(bytes, st, cs, p))
+                      : (a->interleaved ? launch_rotary<__half, true>(bytes, st, cs, p)
+                                        : launch_rotary<__half, false>(bytes, st, cs, p))));
     return RPFQ_OK;
 }
 

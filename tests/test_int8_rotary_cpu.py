@@ -86,7 +86,7 @@ def test_rotary_rejects(bad):
 
 def test_rotary_unsupported_and_empty():
     assert _rotary(dim=8192, pairs=2049) == _lib.RPFQ_ERR_UNSUPPORTED
-    assert _rotary(heads=65536) == _lib.RPFQ_ERR_UNSUPPORTED
+    assert _rotary(heads=(1 << 24) + 1) == _lib.RPFQ_ERR_UNSUPPORTED
     for empty in (dict(batch=0), dict(length=0), dict(heads=0)):
         assert _rotary(x=None, y=None, positions=None, inv_freq=None, **empty) == _lib.RPFQ_OK
 

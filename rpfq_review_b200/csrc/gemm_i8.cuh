@@ -17,6 +17,8 @@
 // alignment is written in order.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm.cuh"
 #include "ptx.cuh"
 
@@ -83,31 +85,25 @@ __device__ __forceinline__ void gelu_log_pair(float& v0, float& v1) {
     f2_unpack(f2_fma(na, f2_pack(ex2_approx(q0), ex2_approx(q1)), f2_pack(v0, v1)), v0, v1);
 }
 
-// The four outputs at (row, col..col + 3), `live` of them inside n.
+// Four outputs of a row, at columns col + e * step (those inside n): the value,
+// activated, plus the residual, rounded once.
 template <bool OUT_F32>
-__device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int live, float (&v)[4]) {
+__device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int step, float (&v)[4]) {
+    using Out = typename std::conditional<OUT_F32, float, __half>::type;
     if (p.activation == kActGelu) {
         gelu_log_pair(v[0], v[1]);
         gelu_log_pair(v[2], v[3]);
     }
-    if constexpr (OUT_F32) {
-        float* y = static_cast<float*>(p.y) + row * p.ldy + col;
-        const float* r = p.residual ? static_cast<const float*>(p.residual) + row * p.ldr + col : nullptr;
-        if (p.vec_out && live == 4) {
+    Out* y = static_cast<Out*>(p.y) + row * p.ldy + col;
+    const Out* r = p.residual ? static_cast<const Out*>(p.residual) + row * p.ldr + col : nullptr;
+    if (p.vec_out && step == 1 && col + 4 <= p.n) {
+        if constexpr (OUT_F32) {
             if (r) {
                 const float4 a = *reinterpret_cast<const float4*>(r);
                 v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
             }
             *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < live) y[e] = v[e] + (r ? r[e] : 0.0f);
-        }
-    } else {
-        __half* y = static_cast<__half*>(p.y) + row * p.ldy + col;
-        const __half* r = p.residual ? static_cast<const __half*>(p.residual) + row * p.ldr + col : nullptr;
-        if (p.vec_out && live == 4) {
             if (r) {
                 const uint2 a = *reinterpret_cast<const uint2*>(r);
                 const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
@@ -115,15 +111,16 @@ __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t 
                 v[0] += a0.x, v[1] += a0.y, v[2] += a1.x, v[3] += a1.y;
             }
             const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
-            uint2 o;
-            o.x = *reinterpret_cast<const uint32_t*>(&h0);
-            o.y = *reinterpret_cast<const uint32_t*>(&h1);
-            *reinterpret_cast<uint2*>(y) = o;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < live) y[e] = __float2half_rn(v[e] + (r ? __half2float(r[e]) : 0.0f));
+            *reinterpret_cast<uint2*>(y) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
         }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e * step >= p.n) break;
+        if (r) v[e] += static_cast<float>(r[e * step]);
+        y[e * step] = static_cast<Out>(v[e]);
     }
 }
 
@@ -227,17 +224,20 @@ __global__ void __launch_bounds__(256)
     // what the outputs need besides the sums is on its way meanwhile
     constexpr int LANES = BN / 4;             // threads of a row, four columns each
     constexpr int STEP = C::THREADS / LANES;  // rows at once
+    // the four columns of a thread: neighbours where rows take vectors of four, else
+    // LANES apart, so that single values of a row are still written side by side
     const int my = threadIdx.x % LANES;
-    const int col = n0 + 4 * my;
-    const int live = p.n - col < 4 ? p.n - col : 4;
+    const int cstep = p.vec_out ? 1 : LANES;
+    const int my_col = p.vec_out ? 4 * my : my;
+    const int col = n0 + my_col;
     float ws[4], b[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        ws[e] = e < live ? __ldg(p.w_scale + col + e) : 0.0f;
+        const int c = col + e * cstep;
+        ws[e] = c < p.n ? __ldg(p.w_scale + c) : 0.0f;
         b[e] = 0.0f;
-        if (p.bias != nullptr && e < live)
-            b[e] = p.bias_f32 ? static_cast<const float*>(p.bias)[col + e]
-                              : __half2float(static_cast<const __half*>(p.bias)[col + e]);
+        if (p.bias != nullptr && c < p.n)
+            b[e] = p.bias_f32 ? static_cast<const float*>(p.bias)[c] : __half2float(static_cast<const __half*>(p.bias)[c]);
     }
     if (threadIdx.x < 128) s_xs[threadIdx.x] = static_cast<int>(threadIdx.x) < rows ? __ldg(p.x_scale + m0 + threadIdx.x) : 0.0f;
     __syncwarp();
@@ -274,35 +274,52 @@ __global__ void __launch_bounds__(256)
     if (warp == 1) tmem_dealloc(tmem_base, BN);
     // ---------------------------------------------------------------- scales, bias, activation, residual
     const int r_lo = split * rows / S, r_hi = (split + 1) * rows / S;
-    if (ok && live > 0) {
+    if (ok && col < p.n) {
         for (int r0 = r_lo + threadIdx.x / LANES; r0 < r_hi; r0 += 4 * STEP) {
-            int4 a[4];
+            int a[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = r0 + i * STEP;
-                if (r < r_hi) a[i] = *reinterpret_cast<const int4*>(staged + r * C::ROW + 4 * my);
-            }
-            if (S > 1) {
-                for (int o = 1; o < S; ++o) {
-                    const uint32_t from = static_cast<uint32_t>(split + o < S ? split + o : split + o - S);
-                    const uint32_t base = mapa_shared(smem_u32(staged + 4 * my), from);
-                    int4 t[4];
+                const int32_t* at = staged + (r0 + i * STEP) * C::ROW + my_col;
+                if (r0 + i * STEP >= r_hi) continue;
+                if (p.vec_out) {
+                    const int4 t = *reinterpret_cast<const int4*>(at);
+                    a[i][0] = t.x, a[i][1] = t.y, a[i][2] = t.z, a[i][3] = t.w;
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (r0 + i * STEP < r_hi) t[i] = ld_shared_cluster_v4(base + (r0 + i * STEP) * C::ROW * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (r0 + i * STEP < r_hi) a[i].x += t[i].x, a[i].y += t[i].y, a[i].z += t[i].z, a[i].w += t[i].w;
+                    for (int e = 0; e < 4; ++e) a[i][e] = at[e * LANES];
                 }
+            }
+            for (int o = 1; o < S; ++o) {
+                const uint32_t from = static_cast<uint32_t>(split + o < S ? split + o : split + o - S);
+                const uint32_t base = mapa_shared(smem_u32(staged + my_col), from);
+                int t[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t at = base + (r0 + i * STEP) * C::ROW * 4;
+                    if (r0 + i * STEP >= r_hi) continue;
+                    if (p.vec_out) {
+                        const int4 u = ld_shared_cluster_v4(at);
+                        t[i][0] = u.x, t[i][1] = u.y, t[i][2] = u.z, t[i][3] = u.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t[i][e] = ld_shared_cluster(at + 4 * e * LANES);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (r0 + i * STEP < r_hi) a[i][e] += t[i][e];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = r0 + i * STEP;
                 if (r >= r_hi) break;
                 const float xs = s_xs[r];
-                float v[4] = {fmaf(__int2float_rn(a[i].x) * ws[0], xs, b[0]), fmaf(__int2float_rn(a[i].y) * ws[1], xs, b[1]),
-                              fmaf(__int2float_rn(a[i].z) * ws[2], xs, b[2]), fmaf(__int2float_rn(a[i].w) * ws[3], xs, b[3])};
-                store_i8_outputs<OUT_F32>(p, m0 + r, col, live, v);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(__int2float_rn(a[i][e]) * ws[e], xs, b[e]);
+                store_i8_outputs<OUT_F32>(p, m0 + r, col, cstep, v);
             }
         }
     }

@@ -114,7 +114,12 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
     return r;
 }
 
-// 16 bytes of shared memory of any CTA of the cluster (shared::cluster address).
+// Shared memory of any CTA of the cluster (shared::cluster address): 4 and 16 bytes.
+__device__ __forceinline__ int ld_shared_cluster(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t addr) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"

@@ -510,14 +510,16 @@ GEMM_INT8_MAX_K = 131071  # 128 * 128 * k < 2^31: the int32 sums cannot overflow
 
 
 def _forward_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
 
 
-def _same_device(name: str, index: int, **tensors) -> None:
-    for what, t in tensors.items():
+def _same_device(name: str, index: int, *tensors) -> None:
+    for t in tensors:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"{name}: {what} is on {t.device}, not on cuda:{index}")
+            raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
 
 
 def _float_type(t: torch.Tensor, name: str) -> bool:
@@ -533,8 +535,9 @@ def _float_type(t: torch.Tensor, name: str) -> bool:
 
 def _matrix(t: torch.Tensor, k: int, name: str):
     """``t[..., k]`` as rows: (tensor to keep, rows, row stride)."""
-    if t.dim() == 0 or t.shape[-1] != k:
-        raise ValueError(f"{name}: last dim of {tuple(t.shape)} is not {k}")
+    shape = t.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"{name}: last dim of {tuple(shape)} is not {k}")
     if t.is_contiguous():
         return t, t.numel() // k, k
     t2, ld = _rows(t, k, name)
@@ -607,7 +610,7 @@ def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x
     w2, _, ldw = _code_rows(w, k, "w")
     w_scale = w_scale.contiguous()
     if out is None:
-        out = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
         ldy = n
     else:
         y2, rows, ldy = _matrix(out, n, "out")
@@ -621,7 +624,7 @@ def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x
         if rows != m:
             raise ValueError(f"{name}: residual rows do not match x")
         r_ptr = r2.data_ptr()
-    _same_device(name, index, w=w, w_scale=w_scale, bias=bias, residual=residual, out=out)
+    _same_device(name, index, w, w_scale, bias, residual, out)
     L = _lib.lib()
     scratch, need = None, 0
     if x_flag:
@@ -664,7 +667,7 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     x2, m, ldx = _code_rows(x, w.shape[1], "x")
     if x_scale.numel() != m:
         raise ValueError(f"{name}: x_scale must hold one value per row ({m}), got {x_scale.numel()}")
-    _same_device(name, x.get_device(), x_scale=x_scale)
+    _same_device(name, x.get_device(), x_scale)
     x_scale = x_scale.contiguous()
     return _gemm_int8(name, x, x2, m, ldx, x_scale.data_ptr(), 0, w, w_scale, bias, residual, activation, out,
                       out_dtype, block_n, split_k)
@@ -793,7 +796,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or (D > 1 and out.stride(-1) != 1):
         raise ValueError(f"{name}: out must not be expanded and must have unit stride inside a head")
     index = x.get_device()
-    _same_device(name, index, positions=positions, inv_freq=inv_freq, out=out)
+    _same_device(name, index, positions, inv_freq, out)
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     xs, ys = x.stride(), out.stride()
     four = len(xs) == 4

@@ -86,6 +86,7 @@ class PackedPhaseLinear(nn.Module):
         # compute="int8": the coefficients as int8 codes [N, K] and fp32 scales [N]
         self.register_buffer("codes8", None, persistent=False)
         self.register_buffer("scale8", None, persistent=False)
+        self._planes8 = None  # the planes (and their versions) that codes8 comes from
         self._bias32 = None  # (version, fp32 copy of bias) for the epilogue
 
     # -- construction ---------------------------------------------------------
@@ -134,6 +135,10 @@ class PackedPhaseLinear(nn.Module):
             self._bias32 = (key, self.bias.float())
         return self._bias32[1]
 
+    def _planes_key(self):
+        return tuple((t.data_ptr(), t._version) for tag in ("u", "w") for s in range(self.stages)
+                     for t in getattr(self, f"{tag}_s{s}")._buffers.values())
+
     @property
     def _fused_decode_ok(self) -> bool:
         # the fused decode path stores 8 complex columns per vector
@@ -154,7 +159,9 @@ class PackedPhaseLinear(nn.Module):
         ``compute="int8"`` the decoded rows are quantized and only their codes
         and scales are kept; returns the codes."""
         if self.compute == "int8":
+            key = self._planes_key()
             self.codes8, self.scale8 = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
+            self._planes8 = key
             return self.codes8
         self.dense = self._decode_dense()
         return self.dense
@@ -173,7 +180,8 @@ class PackedPhaseLinear(nn.Module):
             out_dtype = out.dtype if out is not None else (x.dtype if x.dtype in (torch.float16, torch.float32)
                                                            else torch.float16)
         if self.compute == "int8":
-            if self.codes8 is None or self.codes8.device != x.device:
+            # again after the planes were loaded, written or moved, or the scales cast with the module
+            if self.codes8 is None or self._planes8 != self._planes_key() or self.scale8.dtype != torch.float32:
                 self.prepack()
             xf = x if x.dtype in (torch.float16, torch.float32) else x.to(torch.float16)
             return ops.linear_int8(xf, self.codes8, self.scale8, self._bias_f32(), residual, self.activation, out,

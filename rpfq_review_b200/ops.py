@@ -893,6 +893,29 @@ _LIB.define("wide_linear(Tensor x, Tensor[] codes, Tensor[] gamma_re, Tensor[] g
             "int k_c, int act_bits=0, bool gelu=False) -> Tensor")
 _LIB.define("wide_linear_dense(Tensor x, Tensor dense, Tensor? bias, int n_c, int k_c, int act_bits=0, "
             "int activation=0, Tensor? residual=None) -> Tensor")
+# The 8-bit linear path and the rotary positions (the functions of the same names).
+_LIB.define("quantize_rows(Tensor x) -> (Tensor, Tensor)")
+_LIB.define("gemm_int8(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, Tensor? bias=None, Tensor? residual=None, "
+            "int activation=0, bool out_f32=False) -> Tensor")
+_LIB.define("linear_int8(Tensor x, Tensor w, Tensor w_scale, Tensor? bias=None, Tensor? residual=None, "
+            "int activation=0, bool out_f32=False) -> Tensor")
+_LIB.define("rotary(Tensor x, Tensor positions, Tensor inv_freq, str layout=\"half\", int axes=1, "
+            "float magnitude=1.0, bool transpose=False) -> Tensor")
+
+
+def _op_gemm_int8(x, x_scale, w, w_scale, bias=None, residual=None, activation=0, out_f32=False):
+    return gemm_int8(x, x_scale, w, w_scale, bias, residual, int(activation),
+                     out_dtype=torch.float32 if out_f32 else torch.float16)
+
+
+def _op_linear_int8(x, w, w_scale, bias=None, residual=None, activation=0, out_f32=False):
+    return linear_int8(x, w, w_scale, bias, residual, int(activation),
+                       out_dtype=torch.float32 if out_f32 else torch.float16)
+
+
+def _op_rotary(x, positions, inv_freq, layout="half", axes=1, magnitude=1.0, transpose=False):
+    return rotary(x, positions, inv_freq, layout=layout, axes=int(axes), magnitude=float(magnitude),
+                  transpose=bool(transpose))
 
 
 def _op_gemm(x, w, bias=None, residual=None, activation=0):
@@ -991,6 +1014,10 @@ def _op_wide_linear_dense(x, dense, bias, n_c, k_c, act_bits=0, activation=0, re
 
 _LIB.impl("gemm", _op_gemm, "CUDA")
 _LIB.impl("act_quant", _op_act_quant, "CUDA")
+_LIB.impl("quantize_rows", quantize_rows, "CUDA")
+_LIB.impl("gemm_int8", _op_gemm_int8, "CUDA")
+_LIB.impl("linear_int8", _op_linear_int8, "CUDA")
+_LIB.impl("rotary", _op_rotary, "CUDA")
 _LIB.impl("prepack", _op_prepack, "CUDA")
 _LIB.impl("wide_linear", _op_wide_linear, "CUDA")
 _LIB.impl("wide_linear_dense", _op_wide_linear_dense, "CUDA")

@@ -133,14 +133,15 @@ class PackedViT(nn.Module):
         ntok = 2 if cfg.distilled else 1
         self.register_buffer("cls_tokens", _trunc_normal((1, ntok, d), 0.02, g).half().to(dev))
         self.register_buffer("pos_embed", _trunc_normal((1, cfg.tokens, d), 0.02, g).half().to(dev))
-        self.rotary = None
+        # (frequencies, positions) per device; not buffers: a module cast would round the fp64 angles
+        self.rotary = self._rotary_opts = None
+        self._rotary_tables: dict = {}
         if rotary is not None:
             opts = dict(rotary)
             layout, rot_dim = opts.pop("layout", "half"), opts.pop("rot_dim", d // cfg.heads)
-            inv_freq, magnitude = ops.rotary_frequencies(rot_dim, axes=2, device=dev, **opts)
-            self.rotary = dict(layout=layout, axes=2, magnitude=magnitude)
-            self.register_buffer("rotary_inv_freq", inv_freq, persistent=False)
-            self.register_buffer("rotary_positions", grid_positions(cfg).to(dev), persistent=False)
+            self._rotary_opts = dict(opts, rot_dim=rot_dim, axes=2)
+            self.rotary = dict(layout=layout, axes=2, magnitude=ops.rotary_frequencies(**self._rotary_opts)[1])
+            self._rotary_table(dev)
 
         def make(name, n_out, n_in, activation="none"):
             if weights == "random_init":
@@ -231,6 +232,13 @@ class PackedViT(nn.Module):
             cache[key] = entry
         return entry
 
+    def _rotary_table(self, device: torch.device):
+        key = str(device)
+        if key not in self._rotary_tables:
+            self._rotary_tables[key] = (grid_positions(self.cfg).to(device),
+                                        ops.rotary_frequencies(**self._rotary_opts)[0].to(device))
+        return self._rotary_tables[key]
+
     @torch.no_grad()
     def forward(self, images: torch.Tensor) -> torch.Tensor:
         """images ``[B, 3, 224, 224]`` (already normalised; fp16 or fp32) ->
@@ -270,7 +278,7 @@ class PackedViT(nn.Module):
             qkv = blk.qkv(h, prequantized=pre)
             if self.rotary is not None:  # query and key heads, in place
                 qk = qkv.view(B, L, 3 * H, hd)[:, :, :2 * H]
-                ops.rotary(qk, self.rotary_positions, self.rotary_inv_freq, out=qk, **self.rotary)
+                ops.rotary(qk, *self._rotary_table(qk.device), out=qk, **self.rotary)
             if self.attention == "rpfq" and hd == 64 and L <= ops.ATTENTION_MAX_TOKENS:
                 a = ops.attention(qkv.view(B, L, 3 * d), H)
             else:

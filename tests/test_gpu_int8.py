@@ -356,3 +356,61 @@ def test_gemm_int8_tiles_and_splits_same_bits(cuda, m, n, k):
         assert torch.equal(inplace, want)
     torch.cuda.synchronize()
     assert _lib.device_error() == 0
+
+
+def test_int8_refusals(cuda):
+    from rpfq_review_b200 import ops
+    xq, xs, wq, ws = _operands(cuda, 4, 6, 32)
+    x = torch.randn(4, 32, device=cuda)
+    bad = [
+        lambda: ops.gemm_int8(x, xs, wq, ws), lambda: ops.gemm_int8(xq, xs, x, ws),
+        lambda: ops.gemm_int8(xq, xs.half(), wq, ws), lambda: ops.gemm_int8(xq, xs, wq, ws.double()),
+        lambda: ops.gemm_int8(xq, xs[:3], wq, ws), lambda: ops.gemm_int8(xq, xs, wq, ws[:5]),
+        lambda: ops.gemm_int8(xq[:, :31], xs, wq, ws), lambda: ops.gemm_int8(xq, xs, wq[0], ws),
+        lambda: ops.gemm_int8(xq, xs, wq[:, :0], ws), lambda: ops.gemm_int8(xq, xs, wq, ws, bias=ws[:5]),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, bias=ws.double()), lambda: ops.gemm_int8(xq, xs, wq, ws, bias=ws.cpu()),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, activation="relu"),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, out_dtype=torch.bfloat16),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, out=torch.empty(3, 6, device=cuda)),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, out=torch.empty(4, 5, device=cuda)),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, out=torch.empty(6, 4, device=cuda).t()),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, residual=torch.zeros(3, 6, device=cuda)),
+        lambda: ops.gemm_int8(xq, xs, wq, ws, block_n=32), lambda: ops.gemm_int8(xq, xs, wq, ws, split_k=9),
+        lambda: ops.linear_int8(xq, wq, ws), lambda: ops.linear_int8(x.double(), wq, ws),
+        lambda: ops.linear_int8(x.bfloat16(), wq, ws), lambda: ops.linear_int8(x[:, :31], wq, ws),
+        lambda: ops.linear_int8(x.requires_grad_(), wq, ws), lambda: ops.quantize_rows(x.detach()[:, :0]),
+        lambda: ops.quantize_rows(x.detach().requires_grad_()), lambda: ops.quantize_rows(xq),
+        lambda: ops.quantize_rows(torch.tensor(1.0, device=cuda))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was accepted")
+    with pytest.raises(NotImplementedError):  # residual and output of different types
+        ops.gemm_int8(xq, xs, wq, ws, residual=torch.zeros(4, 6, device=cuda))
+    with torch.no_grad():
+        ops.linear_int8(x, wq, ws)
+    out = torch.ops.rpfq.linear_int8(x.detach(), wq, ws, None, None, 1, True)
+    assert torch.equal(out, ops.linear_int8(x.detach(), wq, ws, activation="gelu", out_dtype=torch.float32))
+    q, s = torch.ops.rpfq.quantize_rows(x.detach())
+    assert torch.equal(torch.ops.rpfq.gemm_int8(q, s, wq, ws, None, None, 1, True), out)
+
+
+def test_gelu_over_its_range(cuda):
+    """The GELU of the product over all magnitudes, infinities and NaN: one code times
+    w_scale gives the argument exactly."""
+    from rpfq_review_b200 import ops
+    v = torch.cat([torch.linspace(-12, 12, 20001), torch.logspace(-30, 30, 600), -torch.logspace(-30, 30, 600),
+                   torch.tensor([float("inf"), float("-inf"), float("nan"), 0.0])])
+    one = torch.ones(1, 1, dtype=torch.int8, device=cuda)
+    w = torch.ones(v.numel(), 1, dtype=torch.int8, device=cuda)
+    for rows in (1, 20, 40000):  # few rows, tiles, CTA pairs
+        n = 21205 if rows < 40000 else 256
+        vv = v[:n] if n == v.numel() else v[:: v.numel() // n][:n]
+        y = ops.gemm_int8(one.expand(rows, 1), torch.ones(rows, device=cuda), w[:n], vv.to(cuda), activation="gelu",
+                          out_dtype=torch.float32)[rows // 2].cpu().double()
+        x = vv.double()
+        ref = x * torch.special.ndtr(x)
+        fin = torch.isfinite(vv)
+        assert ((y - ref).abs()[fin] <= 2.0 ** -20 * x.abs()[fin] + 1e-37).all()
+        if n == v.numel():
+            assert y[-4] == float("inf") and y[-3] == 0 and torch.isnan(y[-2]) and y[-1] == 0

@@ -51,7 +51,7 @@ def _forward_ref(model, images, layout):
     norm = lambda t, w, b: F.layer_norm(t, (d,), w.double(), b.double(), cfg.eps)  # noqa: E731
     for blk in model.blocks:
         qkv = _linear(blk.qkv, norm(x, blk.norm1_w, blk.norm1_b)).view(B, L, 3, H, d // H)
-        q, k = (_turn(qkv[:, :, i], model.rotary_positions, model.rotary_inv_freq, layout) for i in (0, 1))
+        q, k = (_turn(qkv[:, :, i], *model._rotary_table(images.device), layout) for i in (0, 1))
         q, k, v = (t.transpose(1, 2) for t in (q, k, qkv[:, :, 2]))
         a = torch.softmax(q @ k.transpose(-2, -1) / 8.0, -1) @ v
         x = _linear(blk.proj, a.transpose(1, 2).reshape(B, L, d), x)
@@ -84,3 +84,21 @@ def test_int8_rotary_vit(cuda, layout, attention):
     assert torch.equal(z, y)
     assert not torch.equal(PackedViT(_tiny(), cuda, **kw)(images), y)
     assert _lib.device_error() == 0
+
+
+def test_int8_rotary_vit_follows_its_weights(cuda):
+    """Planes loaded into a model that has run, a cast and a move of the module: the codes
+    are those of the planes, the angles stay in 64 bits."""
+    from rpfq_review_b200.vit import PackedViT
+    kw = dict(compute="int8", rotary=dict(base=100.0))
+    a, b = PackedViT(_tiny(), cuda, seed=1, **kw), PackedViT(_tiny(), cuda, seed=2, **kw)
+    images = torch.randn(2, 3, 64, 64, generator=torch.Generator().manual_seed(2)).to(cuda)
+    ya, yb = a(images), b(images)
+    assert not torch.equal(ya, yb)
+    a.load_state_dict(b.state_dict())
+    assert torch.equal(a(images), yb)
+    a.half()
+    assert torch.equal(a(images), yb)
+    a.cpu()
+    a.to(cuda)
+    assert torch.equal(a(images), yb)

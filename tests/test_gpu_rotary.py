@@ -195,3 +195,46 @@ def test_rotary_graph_and_large_offsets(cuda):
     assert torch.equal(far, y)
     torch.cuda.synchronize()
     assert _lib.device_error() == 0
+
+
+def test_rotary_refusals(cuda):
+    from rpfq_review_b200 import ops
+    x, pos, f = torch.randn(2, 5, 3, 16, device=cuda), torch.arange(5, device=cuda), _freq(8)
+    bad = [
+        lambda: ops.rotary(x.double(), pos, f), lambda: ops.rotary(x.bfloat16(), pos, f), lambda: ops.rotary(x[0, 0], pos, f),
+        lambda: ops.rotary(x, pos.cpu(), f), lambda: ops.rotary(x, pos.half(), f), lambda: ops.rotary(x, pos[:4], f),
+        lambda: ops.rotary(x, pos.expand(3, 5), f), lambda: ops.rotary(x[0], pos.expand(1, 5), f),
+        lambda: ops.rotary(x, pos, f.float()), lambda: ops.rotary(x, pos, f.cpu()), lambda: ops.rotary(x, pos, _freq(9)),
+        lambda: ops.rotary(x, pos, f[:0]), lambda: ops.rotary(x, pos, f, axes=2), lambda: ops.rotary(x, pos, f, axes=3),
+        lambda: ops.rotary(x, pos[:, None].expand(5, 2), f[:7], axes=2), lambda: ops.rotary(x, pos, f, layout="pairs"),
+        lambda: ops.rotary(x, pos, f, out=x.half()), lambda: ops.rotary(x, pos, f, out=x[:, :, :2]),
+        lambda: ops.rotary(x, pos, f, out=x[:1].expand(2, 5, 3, 16)), lambda: ops.rotary(x[..., ::2], pos, f[:4], out=x[..., ::2]),
+        lambda: ops.rotary(x.clone().requires_grad_(), pos, f)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was accepted")
+    for empty in (x[:0], x[:, :0], x[:, :, :0]):
+        assert ops.rotary(empty, pos[: empty.shape[1]], f).shape == empty.shape
+    y = torch.ops.rpfq.rotary(x, pos, f, "interleaved", 1, 1.5, True)
+    assert torch.equal(y, ops.rotary(x, pos, f, layout="interleaved", magnitude=1.5, transpose=True))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("B,L,H,D,P", [(1, 3000, 32, 64, 32), (700, 3, 2, 32, 16), (1, 9000, 1, 8, 4), (3, 400, 40, 128, 32),
+                                       (1, 2, 3, 2100, 300), (1, 70, 300, 16, 8)])
+def test_rotary_many_tokens_and_heads(cuda, layout, B, L, H, D, P):
+    """Tokens over many blocks, heads beyond a thread's copies in flight, heads of more
+    pieces than a block has threads."""
+    from rpfq_review_b200 import ops
+    g = torch.Generator().manual_seed(L)
+    f, pos = _freq(P), torch.randint(0, 5000, (B, L), generator=g).to(cuda)
+    for dtype in (torch.float16, torch.float32):
+        x = torch.randn(B, L, H, D, generator=g).to(dtype).to(cuda)
+        ref = _ref(x, pos, f, layout, 1, 1.0, False)
+        _check(ops.rotary(x, pos, f, layout=layout), ref)
+        odd = torch.zeros(B, L, H, D + 1, dtype=dtype, device=cuda)[..., 1:]
+        odd.copy_(x)
+        _check(ops.rotary(odd, pos, f, layout=layout), ref)
+        ops.rotary(x, pos, f, layout=layout, out=x)
+        _check(x, ref)

@@ -85,31 +85,46 @@ __device__ __forceinline__ void gelu_log_pair(float& v0, float& v1) {
     f2_unpack(f2_fma(na, f2_pack(ex2_approx(q0), ex2_approx(q1)), f2_pack(v0, v1)), v0, v1);
 }
 
-// Four outputs of a row, at columns col + e * step (those inside n): the value,
-// activated, plus the residual, rounded once.
+// Four outputs of a row lie at columns col + e * step (those inside n). Their
+// residual (0 without one), to be read for several rows before the first is written:
+// y may be the residual.
 template <bool OUT_F32>
-__device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int step, float (&v)[4]) {
+__device__ __forceinline__ void load_i8_residual(const GemmI8Params& p, int64_t row, int col, int step, float (&r)[4]) {
+    using Out = typename std::conditional<OUT_F32, float, __half>::type;
+    const Out* src = static_cast<const Out*>(p.residual) + row * p.ldr + col;
+    if (p.residual == nullptr) {
+        r[0] = r[1] = r[2] = r[3] = 0.0f;
+    } else if (p.vec_out && step == 1 && col + 4 <= p.n) {
+        if constexpr (OUT_F32) {
+            const float4 a = *reinterpret_cast<const float4*>(src);
+            r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(src);
+            const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
+            const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
+            r[0] = a0.x, r[1] = a0.y, r[2] = a1.x, r[3] = a1.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = col + e * step < p.n ? static_cast<float>(src[e * step]) : 0.0f;
+    }
+}
+
+// The value, activated, plus the residual, rounded once.
+template <bool OUT_F32>
+__device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int step, float (&v)[4],
+                                                 const float (&r)[4]) {
     using Out = typename std::conditional<OUT_F32, float, __half>::type;
     if (p.activation == kActGelu) {
         gelu_log_pair(v[0], v[1]);
         gelu_log_pair(v[2], v[3]);
     }
+    if (p.residual != nullptr) v[0] += r[0], v[1] += r[1], v[2] += r[2], v[3] += r[3];
     Out* y = static_cast<Out*>(p.y) + row * p.ldy + col;
-    const Out* r = p.residual ? static_cast<const Out*>(p.residual) + row * p.ldr + col : nullptr;
     if (p.vec_out && step == 1 && col + 4 <= p.n) {
         if constexpr (OUT_F32) {
-            if (r) {
-                const float4 a = *reinterpret_cast<const float4*>(r);
-                v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-            }
             *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-            if (r) {
-                const uint2 a = *reinterpret_cast<const uint2*>(r);
-                const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
-                const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
-                v[0] += a0.x, v[1] += a0.y, v[2] += a1.x, v[3] += a1.y;
-            }
             const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
             *reinterpret_cast<uint2*>(y) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
@@ -117,11 +132,8 @@ __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t 
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (col + e * step >= p.n) break;
-        if (r) v[e] += static_cast<float>(r[e * step]);
-        y[e * step] = static_cast<Out>(v[e]);
-    }
+    for (int e = 0; e < 4; ++e)
+        if (col + e * step < p.n) y[e * step] = static_cast<Out>(v[e]);
 }
 
 template <int BN, bool OUT_F32>
@@ -276,6 +288,10 @@ __global__ void __launch_bounds__(256)
     const int r_lo = split * rows / S, r_hi = (split + 1) * rows / S;
     if (ok && col < p.n) {
         for (int r0 = r_lo + threadIdx.x / LANES; r0 < r_hi; r0 += 4 * STEP) {
+            float res[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + i * STEP < r_hi) load_i8_residual<OUT_F32>(p, m0 + r0 + i * STEP, col, cstep, res[i]);
             int a[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -319,7 +335,7 @@ __global__ void __launch_bounds__(256)
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = fmaf(__int2float_rn(a[i][e]) * ws[e], xs, b[e]);
-                store_i8_outputs<OUT_F32>(p, m0 + r, col, cstep, v);
+                store_i8_outputs<OUT_F32>(p, m0 + r, col, cstep, v, res[i]);
             }
         }
     }

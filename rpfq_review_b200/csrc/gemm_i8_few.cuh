@@ -178,7 +178,9 @@ __global__ void __launch_bounds__(kFewThreads) gemm_i8_few_kernel(const GemmI8Fe
     if (p.g.bias != nullptr)
         b = p.g.bias_f32 ? static_cast<const float*>(p.g.bias)[col] : __half2float(static_cast<const __half*>(p.g.bias)[col]);
     float v[4] = {fmaf(__int2float_rn(mine) * p.g.w_scale[col], s_scale[r], b), 0.0f, 0.0f, 0.0f};
-    store_i8_outputs<OUT_F32>(p.g, r, col, p.g.n, v);  // one column: the others lie past n
+    float res[4];
+    load_i8_residual<OUT_F32>(p.g, r, col, p.g.n, res);  // one column: the others lie past n
+    store_i8_outputs<OUT_F32>(p.g, r, col, p.g.n, v, res);
 }
 
 }  // namespace rpfq

@@ -13,11 +13,16 @@
 //
 // Bound by memory: each value is read once from DRAM and leaves as one byte. The
 // row stays in registers between its maximum and its codes (KEEP 16-byte vectors
-// per thread; longer rows are read again, from L1 / L2). A warp takes a row; when
-// the rows are too few to fill the GPU or too long for a warp's registers, a block
-// of 256 threads does. The maximum of fp16 rows is taken on half pairs; fl(x s)
-// is rounded by adding 1.5 * 2^23 (half to even, as rint), which leaves the code
-// in the low byte of the sum.
+// per thread). 8, 16 or 32 lanes take a row, the fewest that keep it in 8 vectors
+// each (16 for the longest that a warp takes): what a row costs besides its values
+// (the reduction, a reciprocal, a division) is then shared out over more rows of a
+// warp. 50432 rows of 1024 fp16 values, 155 MB: 31.5 us with a warp per row, 27.8 us
+// so. When the rows are too few to fill the GPU, or too long, a block of 256 threads
+// takes one and reads what it cannot keep again, from L1 / L2.
+// Rows off the 16-byte grid are read in the vectors of the grid all the same; their
+// codes are shifted into place with the next lane's. The maximum of fp16 rows is taken on half pairs; fl(x s) is rounded by adding
+// 1.5 * 2^23 (half to even, as rint), which leaves the code in the low byte of the
+// sum.
 #pragma once
 
 #include "actquant.cuh"
@@ -26,7 +31,6 @@
 namespace rpfq {
 
 constexpr float kQuantRowTiny = 1e-30f;
-constexpr int kQuantRowKeep = 8;  // 16-byte vectors of a row that a thread keeps
 
 struct QuantizeRowsParams {
     const void* x;   // fp16 or fp32 [m, k], row stride ldx
@@ -108,43 +112,60 @@ __device__ __forceinline__ void quant_codes(const float (&f)[N], float s, uint32
     }
 }
 
-// VECTOR: rows of x on 16 bytes and rows of q on QuantVec::N bytes; otherwise
-// vectors are put together value by value. THREADS per row: 32 or 256.
-template <typename T, bool VECTOR, int THREADS>
+// How rows are read: vector by vector with nothing over; with a last vector put
+// together value by value; in the vectors of the 16-byte grid, the codes shifted
+// (parts of a warp only); value by value.
+enum : int { kQuantWhole = 0, kQuantTail = 1, kQuantShift = 2, kQuantSingle = 3 };
+
+// THREADS per row: 8, 16, 32 or 256, each with KEEP vectors in registers.
+template <typename T, int MODE, int THREADS, int KEEP>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeRowsParams p) {
     using V = QuantVec<T>;
     constexpr int N = V::N;
+    static_assert(MODE != kQuantShift || THREADS <= 32, "shifted codes come from the next lane");
     const int tid = threadIdx.x & (THREADS - 1);
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / THREADS) + threadIdx.x / THREADS;
     pdl_wait();
     pdl_launch_dependents();
-    if (row >= p.m) return;  // a whole warp or block
-    const T* __restrict__ x = static_cast<const T*>(p.x) + row * p.ldx;
-    int8_t* __restrict__ q = p.q + row * p.ldq;
-    const int vecs = (p.k + N - 1) / N;
+    const bool live = row < p.m;  // lanes of other rows share the warp's shuffles
+    const T* __restrict__ x = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
+    int8_t* __restrict__ q = p.q + (live ? row : 0) * p.ldq;
+    // vector i holds the values from i N - off on
+    const int off = MODE == kQuantShift ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
+    const int vecs = live ? (p.k + off + N - 1) / N : 0;
+    auto whole = [&](int i) {
+        if (MODE == kQuantWhole) return true;
+        if (MODE == kQuantSingle) return false;
+        return i * N >= off && (i + 1) * N - off <= p.k;
+    };
     auto load = [&](int i) {
         V v;
-        if (VECTOR && (i + 1) * N <= p.k) {
-            v.raw = *reinterpret_cast<const uint4*>(x + i * N);
+        if (whole(i)) {
+            v.raw = *reinterpret_cast<const uint4*>(x + i * N - off);
         } else {
             alignas(16) T e[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) e[j] = i * N + j < p.k ? x[i * N + j] : T(0.0f);
+            for (int j = 0; j < N; ++j) {
+                const int at = i * N - off + j;
+                e[j] = at >= 0 && at < p.k ? x[at] : T(0.0f);
+            }
             v.raw = *reinterpret_cast<const uint4*>(e);
         }
         return v;
     };
-    V kept[kQuantRowKeep];
+    V kept[KEEP];
     float amax = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kQuantRowKeep; ++c)
+    for (int c = 0; c < KEEP; ++c)
         if (tid + c * THREADS < vecs) kept[c] = load(tid + c * THREADS);
 #pragma unroll
-    for (int c = 0; c < kQuantRowKeep; ++c)
+    for (int c = 0; c < KEEP; ++c)
         if (tid + c * THREADS < vecs) amax = max_nan(amax, kept[c].amax());
-    for (int i = tid + kQuantRowKeep * THREADS; i < vecs; i += THREADS) amax = max_nan(amax, load(i).amax());
+    if constexpr (THREADS == 256)
+        for (int i = tid + KEEP * THREADS; i < vecs; i += THREADS) amax = max_nan(amax, load(i).amax());
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = (THREADS < 32 ? THREADS : 32) / 2; o > 0; o >>= 1)
+        amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if constexpr (THREADS == 256) {
         __shared__ float part[8];
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
@@ -153,17 +174,20 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeRowsPa
 #pragma unroll
         for (int w = 1; w < 8; ++w) amax = max_nan(amax, part[w]);
     }
+    if (MODE != kQuantShift && !live) return;
     const QuantScale qs = quant_scale(amax);
-    auto store = [&](int i, const V& v) {
-        uint32_t code[N / 4];
+    constexpr int W = N / 4;  // 32-bit words of codes per vector
+    auto codes = [&](const V& v, uint32_t (&code)[W]) {
         float f[N];
         v.values(f);
         quant_codes<N>(f, qs.s, code);
 #pragma unroll
-        for (int g = 0; g < N / 4; ++g)
+        for (int g = 0; g < W; ++g)
             if (qs.bad) code[g] = 0;
-        if (VECTOR && (i + 1) * N <= p.k) {
-            if constexpr (N == 8)
+    };
+    auto put = [&](int i, const uint32_t (&code)[W]) {  // the codes of values i N ..
+        if (MODE == kQuantWhole || (MODE != kQuantSingle && (i + 1) * N <= p.k)) {
+            if constexpr (W == 2)
                 *reinterpret_cast<uint2*>(q + i * N) = make_uint2(code[0], code[1]);
             else
                 *reinterpret_cast<uint32_t*>(q + i * N) = code[0];
@@ -173,11 +197,49 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeRowsPa
                 if (i * N + j < p.k) q[i * N + j] = static_cast<int8_t>(code[j / 4] >> (8 * (j % 4)));
         }
     };
+    if constexpr (MODE == kQuantShift) {
+        uint32_t code[KEEP + 1][W] = {};
 #pragma unroll
-    for (int c = 0; c < kQuantRowKeep; ++c)
-        if (tid + c * THREADS < vecs) store(tid + c * THREADS, kept[c]);
-    for (int i = tid + kQuantRowKeep * THREADS; i < vecs; i += THREADS) store(i, load(i));
-    if (tid == 0) p.scale[row] = qs.scale;
+        for (int c = 0; c < KEEP; ++c)
+            if (tid + c * THREADS < vecs) codes(kept[c], code[c]);
+        const int next = (threadIdx.x & 31 & ~(THREADS - 1)) | ((tid + 1) & (THREADS - 1));
+#pragma unroll
+        for (int c = 0; c < KEEP; ++c) {
+            // the vector after this one: the next lane's, the first lane's next after the last
+            uint32_t both[2 * W + 1];
+#pragma unroll
+            for (int g = 0; g < W; ++g) {
+                both[g] = code[c][g];
+                both[W + g] = __shfl_sync(0xffffffffu, tid == 0 ? code[c + 1][g] : code[c][g], next);
+            }
+            both[2 * W] = 0;
+            const int words = off / 4, bits = 8 * (off % 4);
+            uint32_t out[W];
+#pragma unroll
+            for (int g = 0; g < W; ++g)
+                out[g] = words == 0 ? __funnelshift_r(both[g], both[g + 1], bits)
+                                    : __funnelshift_r(both[g + 1], both[g + 2], bits);
+            const int i = tid + c * THREADS;
+            if (i < vecs && i * N < p.k) put(i, out);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < KEEP; ++c) {
+            if (tid + c * THREADS < vecs) {
+                uint32_t code[W];
+                codes(kept[c], code);
+                put(tid + c * THREADS, code);
+            }
+        }
+        if constexpr (THREADS == 256) {
+            for (int i = tid + KEEP * THREADS; i < vecs; i += THREADS) {
+                uint32_t code[W];
+                codes(load(i), code);
+                put(i, code);
+            }
+        }
+    }
+    if (live && tid == 0) p.scale[row] = qs.scale;
 }
 
 }  // namespace rpfq

@@ -787,15 +787,29 @@ int gemm(const RpfqGemmArgs* a, cudaStream_t stream, RpfqGemmPlan* dry = nullptr
 }
 
 // ---------------------------------------------------------------- row quantizer
-template <typename T>
-cudaError_t launch_quantize_rows(bool vec, bool block_row, int64_t blocks, cudaStream_t stream,
-                                 const QuantizeRowsParams& p) {
+constexpr int kQuantKeep = 8;  // vectors a thread keeps; twice as many where a warp's 32 lanes need them
+
+template <typename T, int MODE>
+cudaError_t launch_quantize_rows(int threads, bool twice, int64_t blocks, cudaStream_t stream, const QuantizeRowsParams& p) {
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-    if (vec)
-        return block_row ? launch_kernel(quantize_rows_kernel<T, true, 256>, grid, block, 0, stream, 1, p)
-                         : launch_kernel(quantize_rows_kernel<T, true, 32>, grid, block, 0, stream, 1, p);
-    return block_row ? launch_kernel(quantize_rows_kernel<T, false, 256>, grid, block, 0, stream, 1, p)
-                     : launch_kernel(quantize_rows_kernel<T, false, 32>, grid, block, 0, stream, 1, p);
+    if (threads == 8) return launch_kernel(quantize_rows_kernel<T, MODE, 8, kQuantKeep>, grid, block, 0, stream, 1, p);
+    if (threads == 16) return launch_kernel(quantize_rows_kernel<T, MODE, 16, kQuantKeep>, grid, block, 0, stream, 1, p);
+    if (twice) return launch_kernel(quantize_rows_kernel<T, MODE, 32, 2 * kQuantKeep>, grid, block, 0, stream, 1, p);
+    return launch_kernel(quantize_rows_kernel<T, MODE, 32, kQuantKeep>, grid, block, 0, stream, 1, p);
+}
+
+template <typename T>
+cudaError_t launch_quantize_rows(int mode, int threads, bool twice, int64_t blocks, cudaStream_t stream,
+                                 const QuantizeRowsParams& p) {
+    if (threads == 256) {
+        const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+        if (mode == kQuantWhole || mode == kQuantTail)
+            return launch_kernel(quantize_rows_kernel<T, kQuantTail, 256, kQuantKeep>, grid, block, 0, stream, 1, p);
+        return launch_kernel(quantize_rows_kernel<T, kQuantSingle, 256, kQuantKeep>, grid, block, 0, stream, 1, p);
+    }
+    if (mode == kQuantWhole) return launch_quantize_rows<T, kQuantWhole>(threads, twice, blocks, stream, p);
+    if (mode == kQuantTail) return launch_quantize_rows<T, kQuantTail>(threads, twice, blocks, stream, p);
+    return launch_quantize_rows<T, kQuantShift>(threads, twice, blocks, stream, p);
 }
 
 // Checked arguments; the caller has set up the device.
@@ -809,15 +823,21 @@ int quantize_rows(const char* who, const void* x, bool f32, int64_t ldx, int8_t*
     p.scale = scale;
     p.m = m;
     p.k = k;
-    // a block per row when warps would not fill the GPU or keep the row
-    const int esize = f32 ? 4 : 2;
-    const bool block_row = m < int64_t(8) * st->sm_count || int64_t(k) * esize > 32 * 16 * kQuantRowKeep;
-    const int64_t blocks = block_row ? m : (m + 7) / 8;
+    // rows of x on 16 bytes, nothing over in the last vector; codes on their vectors' words
+    const int esize = f32 ? 4 : 2, n = 16 / esize;
+    const bool grid16 = aligned16(x) && ldx * esize % 16 == 0;
+    const bool words = reinterpret_cast<uintptr_t>(q) % n == 0 && ldq % n == 0;
+    const int mode = !words ? kQuantSingle : (!grid16 ? kQuantShift : (k % n ? kQuantTail : kQuantWhole));
+    // a block per row when parts of warps would not fill the GPU or keep the row
+    const int64_t vecs = (static_cast<int64_t>(k) + (mode == kQuantShift ? 2 * n - 2 : n - 1)) / n;
+    int threads = 8;
+    while (threads < 32 && vecs > threads * kQuantKeep) threads *= 2;
+    const bool twice = vecs > 32 * kQuantKeep;
+    if (vecs > 64 * kQuantKeep || mode == kQuantSingle || m * threads < int64_t(256) * st->sm_count) threads = 256;
+    const int64_t blocks = (m * threads + 255) / 256;
     if (blocks > 0x7fffffff || k > (1 << 30)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or k too large", who);
-    const int qvec = 16 / esize;
-    const bool vec = aligned16(x) && ldx * esize % 16 == 0 && reinterpret_cast<uintptr_t>(q) % qvec == 0 && ldq % qvec == 0;
-    RPFQ_CUDA((f32 ? launch_quantize_rows<float>(vec, block_row, blocks, stream, p)
-                   : launch_quantize_rows<__half>(vec, block_row, blocks, stream, p)));
+    RPFQ_CUDA((f32 ? launch_quantize_rows<float>(mode, threads, twice, blocks, stream, p)
+                   : launch_quantize_rows<__half>(mode, threads, twice, blocks, stream, p)));
     return RPFQ_OK;
 }
 

@@ -70,7 +70,10 @@ def _operands(dev, m, n, k, seed=0, full_range=False):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 7), (5, 8), (9, 100), (33, 768), (2, 4096), (300, 1003), (4, 20011)])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 7), (5, 8), (9, 100), (33, 768), (2, 4096), (300, 1003), (4, 20011),
+                                 (5003, 64), (4801, 33), (2500, 1024), (2501, 516), (1301, 2048), (1301, 1030), (1300, 2056),
+                                 (5000, 1), (4900, 7), (4900, 62), (2500, 129), (2500, 1017), (1300, 4090), (1300, 1999),
+                                 (1300, 4097)])
 def test_quantize_rows_bit_exact(cuda, dtype, m, k):
     from rpfq_review_b200 import ops
     g = torch.Generator().manual_seed(m * 31 + k)
@@ -84,6 +87,22 @@ def test_quantize_rows_bit_exact(cuda, dtype, m, k):
     # half a code, and the fp32 roundings of x s (|x s| <= 127) and of the scale
     bound = scale.cpu().double().unsqueeze(1) * (0.5 + 127 * 4 * U)
     assert ((back - x.double()).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_quantize_rows_off_the_grid(cuda, dtype):
+    """Rows that start at every offset from 16 bytes, with strides of every remainder."""
+    from rpfq_review_b200 import ops
+    g = torch.Generator().manual_seed(0)
+    flat = torch.randn(5000 * 90, generator=g).to(dtype)
+    flat[7::1013] = float("nan")
+    dev = flat.to(cuda)
+    for k in (1, 5, 30, 64, 67):
+        for stride in range(k, k + 9):
+            for start in (0, 1, 3):
+                want_q, want_s = _codes_ref(flat.as_strided((4800, k), (stride, 1), start).float().numpy())
+                q, s = ops.quantize_rows(dev.as_strided((4800, k), (stride, 1), start))
+                assert np.array_equal(q.cpu().numpy(), want_q) and np.array_equal(s.cpu().numpy(), want_s, equal_nan=True)
 
 
 def test_quantize_rows_edges_and_strides(cuda):

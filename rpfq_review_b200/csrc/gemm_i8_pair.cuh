@@ -16,16 +16,25 @@
 // biased in packed fp32 pairs.
 // The accumulator is released as soon as the warp's last part of it is in
 // registers, by an arrival without release semantics: a release waits for the
-// warp's other memory traffic, which the MMA warp does not read.
+// warp's other memory traffic, which the MMA warp does not read (m = 50432, k =
+// 1024, n = 4096: 150 us without GELU against 174..191 with a release).
+//
+// The loops of warps 0 and 1 run on all lanes with only the issuing instruction
+// predicated. On one lane the MMA warp took over 800 cycles for the instructions of
+// a k-block while the epilogue competed for its scheduler; a k-block takes 512.
 //
 // Output and residual steps go through the warp's 128-B-swizzled staging slots by
 // TMA when their addresses and row strides are multiples of 16 bytes, and by
 // row-wise loads and stores of the warp otherwise (n odd). With a residual there
 // are two slots: the next step's residual lands while this one is used.
 //
-// EW: eight epilogue warps, or sixteen for GELU without a residual (two warps per
-// scheduler do not keep up with its two special-function results per value; the
-// price is one stage of the ring).
+// EW: eight epilogue warps, or sixteen for GELU without a residual, at the price of
+// one stage of the ring (177 against 190 us at that size).
+//
+// Bound by the power-capped tensor cores for long k (m = 50432, k = 4096, n = 1024,
+// fp16 out: 135 us, 3.1 POPS, the tensor pipe busy in 98 % of the cycles), by
+// the GELU's instructions for k = 1024, by the residual stream beside them for
+// fp32 in and out (160 us).
 //
 // The last wave of tiles, where at most half full, is cut into column pieces
 // (Schedule, gemm.cuh).
@@ -351,23 +360,28 @@ __global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
                     if (lane == 0) bulk_wait_group_read<0>();
                     __syncwarp();
                 }
-                // 32 columns at a time; a thread reads and writes its own row of the slot only
+                // a few columns at a time (with sixteen warps 16: 32 left the GELU's constants no
+                // registers); a thread reads and writes its own row of the slot only
+                constexpr int CB = EW == 16 ? 16 : 32;
 #pragma unroll
-                for (int h = 0; h < CW / 32; ++h) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(t_row + c * CW + 32 * h, r);
+                for (int h = 0; h < CW / CB; ++h) {
+                    uint32_t r[CB];
+                    if constexpr (CB == 32)
+                        tmem_ld_32x32b_x32(t_row + c * CW + CB * h, r);
+                    else
+                        tmem_ld_32x32b_x16(t_row + c * CW + CB * h, r);
                     tmem_ld_wait(r);
-                    if (c + 1 == nsteps && h + 1 == CW / 32) {
+                    if (c + 1 == nsteps && h + 1 == CW / CB) {
                         // this warp has read its part of the accumulator into registers
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster_relaxed(acc ? tempty_leader1 : tempty_leader0);
                     }
-                    float v[32];
+                    float v[CB];
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const float4 sw = *reinterpret_cast<const float4*>(s_ws + c * CW + 32 * h + 4 * g);
-                        const float4 sb = *reinterpret_cast<const float4*>(s_b + c * CW + 32 * h + 4 * g);
+                    for (int g = 0; g < CB / 4; ++g) {
+                        const float4 sw = *reinterpret_cast<const float4*>(s_ws + c * CW + CB * h + 4 * g);
+                        const float4 sb = *reinterpret_cast<const float4*>(s_b + c * CW + CB * h + 4 * g);
                         const uint64_t a0 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g])),
                                                     __int2float_rn(static_cast<int>(r[4 * g + 1])));
                         const uint64_t a1 = f2_pack(__int2float_rn(static_cast<int>(r[4 * g + 2])),
@@ -379,7 +393,7 @@ __global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
                     }
                     if (p.activation == kActGelu) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) gelu_log_pair(v[e], v[e + 1]);
+                        for (int e = 0; e < CB; e += 2) gelu_log_pair(v[e], v[e + 1]);
                     }
                     if constexpr (RES) {
                         if (h == 0 && p.vec_res) {
@@ -389,8 +403,8 @@ __global__ void __launch_bounds__(GemmI8PairCfg<RES, EW>::THREADS, 1)
                         }
                     }
 #pragma unroll
-                    for (int g = 0; g < 32 / PER; ++g) {
-                        uint4* at = granule(lane, h * (32 / PER) + g);
+                    for (int g = 0; g < CB / PER; ++g) {
+                        uint4* at = granule(lane, h * (CB / PER) + g);
                         float* e = v + PER * g;
                         if constexpr (RES) {
                             const uint4 a = *at;

@@ -587,24 +587,25 @@ def quantize_rows(x: torch.Tensor):
     return (codes if ld == k else codes[..., :k]), scale
 
 
-def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x_scale, x_flag: int, w: torch.Tensor,
-               w_scale: torch.Tensor, bias, residual, activation, out, out_dtype, block_n, split_k) -> torch.Tensor:
+def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x_scale, x_flag: int,
+               w: torch.Tensor, w_scale: torch.Tensor, bias, residual, activation, out, out_dtype, block_n,
+               split_k) -> torch.Tensor:
     """What gemm_int8 and linear_int8 share: the checks of everything but x, and the launch."""
-    index = x.get_device()
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            return _gemm_int8(name, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
+            return _gemm_int8(name, index, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
                               out_dtype, block_n, split_k)
+    _forward_only(name, w_scale, residual)
+    _same_device(name, index, w, w_scale, bias, residual, out)
     n, k = w.shape
-    _require(w_scale, "w_scale", torch.float32)
-    if w_scale.numel() != n:
-        raise ValueError(f"{name}: w_scale must hold {n} values, got {w_scale.numel()}")
+    if w_scale.dtype is not torch.float32 or w_scale.numel() != n:
+        raise ValueError(f"{name}: w_scale must hold {n} float32 values, got {w_scale.numel()} of {w_scale.dtype}")
     if activation not in _ACT:
         raise ValueError(f"{name}: unknown activation {activation!r}")
     bias_ptr = None
     if bias is not None:
-        if not bias.is_cuda or bias.numel() != n:
-            raise ValueError(f"{name}: bias must be a CUDA tensor of {n} values")
+        if bias.numel() != n:
+            raise ValueError(f"{name}: bias must hold {n} values, got {bias.numel()}")
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
     w2, _, ldw = _code_rows(w, k, "w")
@@ -618,19 +619,16 @@ def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x
             raise ValueError(f"{name}: out must be a row-major view of {m} rows with unit column stride")
     r2, ldr, r_ptr = None, 0, None
     if residual is not None:
-        if not residual.is_cuda:
-            raise ValueError(f"{name}: residual must be a CUDA tensor")
         r2, rows, ldr = _matrix(residual, n, "residual")
         if rows != m:
             raise ValueError(f"{name}: residual rows do not match x")
         r_ptr = r2.data_ptr()
-    _same_device(name, index, w, w_scale, bias, residual, out)
     L = _lib.lib()
     scratch, need = None, 0
     if x_flag:
         need = m * ((k + 15) // 16 * 16 + 4) if block_n or split_k else L.rpfq_gemm_i8_scratch_bytes(m, k)
         if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+            scratch = x.new_empty(need, dtype=torch.uint8)
     a = _lib.RpfqGemmI8Args(x2.data_ptr(), ldx, x_scale, w2.data_ptr(), ldw, w_scale.data_ptr(), bias_ptr, r_ptr, ldr,
                             out.data_ptr(), ldy, m, n, k, _ACT[activation], x_flag | _flags(out, r2, bias),
                             block_n, split_k, _p(scratch), need)
@@ -641,9 +639,8 @@ def _gemm_int8(name: str, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x
 
 
 def _check_codes(name: str, w: torch.Tensor) -> None:
-    _require(w, "w", torch.int8)
-    if w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0:
-        raise ValueError(f"{name}: w must be [n, k] with n, k > 0, got {tuple(w.shape)}")
+    if w.dtype is not torch.int8 or w.dim() != 2 or w.numel() == 0:
+        raise ValueError(f"{name}: w must be int8 [n, k] with n, k > 0, got {w.dtype} {tuple(w.shape)}")
 
 
 def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -662,14 +659,15 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     name = "gemm_int8"
     _require(x, "x", torch.int8)
     _check_codes(name, w)
-    _require(x_scale, "x_scale", torch.float32)
-    _forward_only(name, x_scale, w_scale, residual)
+    index = x.get_device()
+    _forward_only(name, x_scale)
+    _same_device(name, index, x_scale)
     x2, m, ldx = _code_rows(x, w.shape[1], "x")
-    if x_scale.numel() != m:
-        raise ValueError(f"{name}: x_scale must hold one value per row ({m}), got {x_scale.numel()}")
-    _same_device(name, x.get_device(), x_scale)
+    if x_scale.dtype is not torch.float32 or x_scale.numel() != m:
+        raise ValueError(f"{name}: x_scale must hold one float32 value per row ({m}), got {x_scale.numel()} of "
+                         f"{x_scale.dtype}")
     x_scale = x_scale.contiguous()
-    return _gemm_int8(name, x, x2, m, ldx, x_scale.data_ptr(), 0, w, w_scale, bias, residual, activation, out,
+    return _gemm_int8(name, index, x, x2, m, ldx, x_scale.data_ptr(), 0, w, w_scale, bias, residual, activation, out,
                       out_dtype, block_n, split_k)
 
 
@@ -683,10 +681,10 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     name = "linear_int8"
     x_flag = _lib.GEMM_X_F32 if _float_type(x, "x") else _lib.GEMM_X_F16
     _check_codes(name, w)
-    _forward_only(name, x, w_scale, residual)
+    _forward_only(name, x)
     x2, m, ldx = _matrix(x, w.shape[1], "x")
-    return _gemm_int8(name, x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out, out_dtype,
-                      block_n, split_k)
+    return _gemm_int8(name, x.get_device(), x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out,
+                      out_dtype, block_n, split_k)
 
 
 # ---------------------------------------------------------------------------

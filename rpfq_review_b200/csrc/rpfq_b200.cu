@@ -1066,6 +1066,19 @@ I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
     return best;
 }
 
+// Whether some row of one matrix shares bytes with some row of another: `rows` rows of
+// a_bytes / b_bytes at strides a_step / b_step bytes. Exact for equal strides (columns
+// of one buffer), by their whole ranges otherwise.
+bool rows_overlap(const void* a, int64_t a_step, int64_t a_bytes, const void* b, int64_t b_step, int64_t b_bytes,
+                  int64_t rows) {
+    const intptr_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+    const int64_t a_all = (rows - 1) * a_step + a_bytes, b_all = (rows - 1) * b_step + b_bytes;
+    if (pa + a_all <= pb || pb + b_all <= pa) return false;
+    if (a_step != b_step || rows == 1) return true;
+    const int64_t shift = ((pb - pa) % a_step + a_step) % a_step;  // b's columns within a's rows
+    return shift < a_bytes || shift + b_bytes > a_step;
+}
+
 int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     const char* who = "rpfq_gemm_i8_sm100";
     if (!args) return fail(RPFQ_ERR_INVALID, "%s: null args", who);
@@ -1101,6 +1114,10 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
     if (a->residual && (((a->flags & RPFQ_GEMM_RESIDUAL_F32) != 0) != ((a->flags & RPFQ_GEMM_OUT_F32) != 0)))
         return fail(RPFQ_ERR_UNSUPPORTED, "%s: the residual must have the output's dtype", who);
+    // rows of x are read until the last output is written
+    if (rows_overlap(a->x, a->ldx * static_cast<int64_t>(xsize), a->k * static_cast<int64_t>(xsize), a->y,
+                     a->ldy * static_cast<int64_t>(esize), a->n * static_cast<int64_t>(esize), a->m))
+        return fail(RPFQ_ERR_INVALID, "%s: y must not overlap x", who);
     if (a->block_n != 0 && a->block_n != 64 && a->block_n != 128 && a->block_n != 256)
         return fail(RPFQ_ERR_INVALID, "%s: block_n must be 0, 64, 128 or 256 (got %d)", who, a->block_n);
     if (a->split_k < 0 || a->split_k > kMaxSplits || (a->split_k > 1 && a->block_n == 256))

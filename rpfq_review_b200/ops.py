@@ -540,6 +540,10 @@ def _matrix(t: torch.Tensor, k: int, name: str):
         raise ValueError(f"{name}: last dim of {tuple(shape)} is not {k}")
     if t.is_contiguous():
         return t, t.numel() // k, k
+    if len(shape) == 2:
+        ld, step = t.stride()
+        if step == 1 and ld >= k:
+            return t, shape[0], ld
     t2, ld = _rows(t, k, name)
     if ld < k:  # rows that overlap (expanded): one copy
         t2, ld = t2.contiguous(), k
@@ -652,8 +656,9 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     channel (``rpfq_gemm_i8_sm100``): exact int32 sums on the tensor cores
     (k up to ``GEMM_INT8_MAX_K``), scaled in fp32. ``bias`` fp16 or fp32;
     ``residual`` and ``out`` fp16 or fp32 alike (and may be the same tensor for
-    an in-place residual add). Code rows that do not start on 16 bytes are
-    copied into rows that do; :func:`quantize_rows` returns such rows.
+    an in-place residual add; ``out`` must not overlap ``x``). Code rows that do
+    not start on 16 bytes are copied into rows that do; :func:`quantize_rows`
+    returns such rows.
     ``block_n`` (64, 128, 256) and ``split_k`` (1..8) fix the tiles and the parts
     of k, 0 leaves them to the library; the result is the same bit for bit."""
     name = "gemm_int8"

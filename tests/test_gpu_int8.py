@@ -433,3 +433,49 @@ def test_gelu_over_its_range(cuda):
         assert ((y - ref).abs()[fin] <= 2.0 ** -20 * x.abs()[fin] + 1e-37).all()
         if n == v.numel():
             assert y[-4] == float("inf") and y[-3] == 0 and torch.isnan(y[-2]) and y[-1] == 0
+
+
+def test_int8_vectors_and_shared_buffers(cuda):
+    """One-dimensional inputs, a broadcast residual, input and output columns of one
+    buffer; an output over its own input is refused."""
+    from rpfq_review_b200 import ops
+    w, ws = ops.quantize_rows(torch.randn(48, 64, device=cuda))
+    x = torch.randn(40, 64, device=cuda)
+    y = ops.linear_int8(x, w, ws, out_dtype=torch.float32)
+    assert torch.equal(ops.linear_int8(x[3], w, ws, out_dtype=torch.float32), y[3])
+    q, s = ops.quantize_rows(x[3])
+    assert q.shape == (64,) and s.shape == ()
+    assert torch.equal(ops.gemm_int8(q, s, w, ws, out_dtype=torch.float32), y[3])
+    assert torch.equal(ops.linear_int8(x.t().contiguous().t()[5], w, ws, out_dtype=torch.float32), y[5])
+    row = torch.randn(48, device=cuda)
+    assert torch.equal(ops.linear_int8(x, w, ws, residual=row.expand(40, 48), out_dtype=torch.float32),
+                       ops.linear_int8(x, w, ws, residual=row.repeat(40, 1), out_dtype=torch.float32))
+    for rows in (2, 40):
+        both = torch.zeros(rows, 112, device=cuda)
+        both[:, :64] = x[:rows]
+        ops.linear_int8(both[:, :64], w, ws, out=both[:, 64:])
+        assert torch.equal(both[:, 64:], y[:rows]) and torch.equal(both[:, :64], x[:rows])
+        with pytest.raises(ValueError, match="overlap"):
+            ops.linear_int8(both[:, :64], w, ws, out=both[:, 40:88])
+
+
+def test_int8_past_31_bits(cuda):
+    """Rows whose elements lie past 2^31: the last ones equal a small call's, in place too."""
+    from rpfq_review_b200 import _lib, ops
+    m, n, k = 530000, 4100, 32
+    x, xs = ops.quantize_rows(torch.randn(m, k, device=cuda))
+    w, ws = ops.quantize_rows(torch.randn(n, k, device=cuda))
+    y = ops.gemm_int8(x, xs, w, ws)  # 2.17e9 elements
+    assert torch.equal(y[-300:], ops.gemm_int8(x[-300:], xs[-300:], w, ws))
+    ops.gemm_int8(x, xs, w, ws, residual=y, out=y)
+    assert torch.equal(y[-300:], ops.gemm_int8(x[-300:], xs[-300:], w, ws, residual=ops.gemm_int8(x[-300:], xs[-300:], w, ws)))
+    q, s = ops.quantize_rows(y)
+    want = ops.quantize_rows(y[-3:])
+    assert torch.equal(q[-3:], want[0]) and torch.equal(s[-3:], want[1])
+    del q
+    far = y.view(-1)[: 129 * 16_800_000].view(129, 16_800_000)[:, -64:]  # rows 33.6 MB apart: the tile kernel
+    out = far[:, :40]
+    ops.gemm_int8(x[:129], xs[:129], w[:40], ws[:40], out=out)
+    assert torch.equal(out, ops.gemm_int8(x[:129], xs[:129], w[:40], ws[:40]))
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0

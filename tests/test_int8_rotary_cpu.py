@@ -21,7 +21,7 @@ def test_struct_sizes():
 
 
 def _gemm(**kw):
-    a = dict(x=A, ldx=64, x_scale=A, w=A, ldw=64, w_scale=A, bias=None, residual=None, ldr=0, y=A, ldy=32, m=4, n=32,
+    a = dict(x=A, ldx=64, x_scale=A, w=A, ldw=64, w_scale=A, bias=None, residual=None, ldr=0, y=2 * A, ldy=32, m=4, n=32,
              k=60, activation=0, flags=0)
     a.update(kw)
     return _lib.lib().rpfq_gemm_i8_sm100(ctypes.byref(_lib.RpfqGemmI8Args(**a)), None)
@@ -30,7 +30,7 @@ def _gemm(**kw):
 @pytest.mark.parametrize("bad", [
     dict(m=-1), dict(n=0), dict(k=0), dict(k=-4), dict(x=None), dict(w=None), dict(y=None), dict(x_scale=None),
     dict(w_scale=None), dict(ldx=48), dict(ldx=72), dict(ldw=48), dict(ldw=60), dict(x=A + 8), dict(w=A + 1),
-    dict(ldy=31), dict(residual=A, ldr=31), dict(y=A + 1), dict(y=A + 2, flags=1), dict(bias=A + 1),
+    dict(ldy=31), dict(residual=A, ldr=31), dict(y=2 * A + 1), dict(y=2 * A + 2, flags=1), dict(bias=A + 1),
     dict(bias=A + 2, flags=4), dict(residual=A + 1, ldr=32), dict(x_scale=A + 2), dict(w_scale=A + 1),
     dict(flags=32), dict(flags=24), dict(activation=2), dict(activation=-1),
     dict(block_n=96), dict(block_n=-1), dict(split_k=9), dict(split_k=-1), dict(block_n=256, split_k=2),
@@ -39,6 +39,19 @@ def _gemm(**kw):
 def test_gemm_i8_rejects(bad):
     assert _gemm(**bad) == _lib.RPFQ_ERR_INVALID
     assert _lib.lib().rpfq_last_error()
+
+
+def test_gemm_i8_refuses_an_output_over_its_input():
+    """x [4, 60] int8 at A, rows of 64 bytes: y over its range, its tail, around it; columns
+    beside x in rows of the same stride pass this check (and fail later, without a GPU)."""
+    for y, ldy, n in ((A, 32, 32), (A + 192, 32, 32), (A - 64, 32, 8), (A + 56, 32, 8), (A + 30, 32, 4)):
+        assert _gemm(y=y, ldy=ldy, n=n) == _lib.RPFQ_ERR_INVALID
+        assert b"overlap" in _lib.lib().rpfq_last_error()
+    wide = dict(ldx=128, ldy=64)  # rows of 128 bytes: x in the first 60, y in the last 64
+    for y, n in ((A + 64, 32), (A + 60, 34)):
+        assert _gemm(y=y, n=n, **wide) == _lib.RPFQ_OK or b"overlap" not in _lib.lib().rpfq_last_error()
+    assert _gemm(y=A + 64, n=33, **wide) == _lib.RPFQ_ERR_INVALID and b"overlap" in _lib.lib().rpfq_last_error()
+    assert _gemm(y=A + 58, n=8, **wide) == _lib.RPFQ_ERR_INVALID and b"overlap" in _lib.lib().rpfq_last_error()
 
 
 def test_gemm_i8_unsupported_and_empty():

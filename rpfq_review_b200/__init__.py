@@ -9,8 +9,9 @@ Public API:
 * :class:`PackedPhaseLinear` — the layer over the exporter's packed layout.
 * :mod:`rpfq_review_b200.ops` — ``prepack`` (K1 decode), ``gemm`` (K2
   tcgen05 GEMM), ``wide_linear`` (dense or fused decode), ``act_quant``,
-  ``vision_act_quant``, ``layernorm``, ``pack_linear`` (GPU packer) and
-  ``torch.ops.rpfq.*``.
+  ``vision_act_quant``, ``layernorm``, ``pack_linear`` (GPU packer), the
+  8-bit linear path (``quantize_rows``, ``gemm_int8``, ``linear_int8``),
+  ``rotary`` positions and ``torch.ops.rpfq.*``.
 * :mod:`rpfq_review_b200.packing` — layout, packer, seeded synthetic layers.
 
 The CUDA library (``librpfq_b200.so``, C ABI in ``include/rpfq_b200.h``) is

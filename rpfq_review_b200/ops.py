@@ -1,7 +1,9 @@
 """PyTorch entry points over the C ABI (``include/rpfq_b200.h``).
 
 Functional wrappers (:func:`prepack`, :func:`gemm`, :func:`act_quant`,
-:func:`wide_linear`) and the ``torch.ops.rpfq`` operators, registered with
+:func:`wide_linear`, the 8-bit linear path :func:`quantize_rows`,
+:func:`gemm_int8`, :func:`linear_int8`, and :func:`rotary` positions) and the
+``torch.ops.rpfq`` operators, registered with
 ``torch.library`` in the same way the reference registers its GPU op
 (``Library("quant", "DEF")`` + ``define`` + ``impl``,
 RPFQ-ViT-main/quant_models/kernel.py:599-605). Every op has a CUDA

@@ -28,8 +28,8 @@
 // row-wise loads and stores of the warp otherwise (n odd). With a residual there
 // are two slots: the next step's residual lands while this one is used.
 //
-// EW: eight epilogue warps, or sixteen for GELU without a residual, at the price of
-// one stage of the ring (177 against 190 us at that size).
+// EW: eight epilogue warps, or sixteen (without a residual) at the price of one stage
+// of the ring; rpfq_b200.cu says when, with both sides measured.
 //
 // Bound by the power-capped tensor cores for long k (m = 50432, k = 4096, n = 1024,
 // fp16 out: 135 us, 3.1 POPS, the tensor pipe busy in 98 % of the cycles), by

@@ -1179,7 +1179,13 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     const I8Plan plan = plan_i8(a, st);
     if (plan.bn == 256) {
         if (res) return f32 ? launch_i8_pair<true, true, 8>(a, p, st, stream) : launch_i8_pair<false, true, 8>(a, p, st, stream);
-        if (p.activation == RPFQ_ACT_GELU)
+        // sixteen epilogue warps where eight do not keep up with the main loop (us, eight /
+        // sixteen at m x n x k): GELU (50432 x 4096 x 1024 190 / 177), rows without TMA
+        // stores (20000 x 1001 x 700 fp16 33 / 29, fp32 41 / 32), fp16 rows of a short main
+        // loop (50432 x 1152 x 384 36 / 31; x 640 38.9 / 38.3); else the ring's sixth stage
+        // is worth more (50432 x 2304 x 1024 fp32 114 / 121, 3152 x 768 x 768 6.2 / 6.8)
+        const bool tma_out = aligned16(a->y) && a->ldy * static_cast<int64_t>(esize) % 16 == 0;
+        if (p.activation == RPFQ_ACT_GELU || !tma_out || (!f32 && a->k <= 512))
             return f32 ? launch_i8_pair<true, false, 16>(a, p, st, stream) : launch_i8_pair<false, false, 16>(a, p, st, stream);
         return f32 ? launch_i8_pair<true, false, 8>(a, p, st, stream) : launch_i8_pair<false, false, 8>(a, p, st, stream);
     }

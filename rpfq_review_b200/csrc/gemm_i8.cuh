@@ -86,15 +86,13 @@ __device__ __forceinline__ void gelu_log_pair(float& v0, float& v1) {
 }
 
 // Four outputs of a row lie at columns col + e * step (those inside n). Their
-// residual (0 without one), to be read for several rows before the first is written:
-// y may be the residual.
-template <bool OUT_F32>
+// residual, to be read for several rows before the first is written: y may be the
+// residual.
+template <bool OUT_F32, bool VEC>
 __device__ __forceinline__ void load_i8_residual(const GemmI8Params& p, int64_t row, int col, int step, float (&r)[4]) {
     using Out = typename std::conditional<OUT_F32, float, __half>::type;
     const Out* src = static_cast<const Out*>(p.residual) + row * p.ldr + col;
-    if (p.residual == nullptr) {
-        r[0] = r[1] = r[2] = r[3] = 0.0f;
-    } else if (p.vec_out && step == 1 && col + 4 <= p.n) {
+    if (VEC && col + 4 <= p.n) {
         if constexpr (OUT_F32) {
             const float4 a = *reinterpret_cast<const float4*>(src);
             r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
@@ -111,7 +109,7 @@ __device__ __forceinline__ void load_i8_residual(const GemmI8Params& p, int64_t 
 }
 
 // The value, activated, plus the residual, rounded once.
-template <bool OUT_F32>
+template <bool OUT_F32, bool RES, bool VEC>
 __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t row, int col, int step, float (&v)[4],
                                                  const float (&r)[4]) {
     using Out = typename std::conditional<OUT_F32, float, __half>::type;
@@ -119,9 +117,9 @@ __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t 
         gelu_log_pair(v[0], v[1]);
         gelu_log_pair(v[2], v[3]);
     }
-    if (p.residual != nullptr) v[0] += r[0], v[1] += r[1], v[2] += r[2], v[3] += r[3];
+    if constexpr (RES) v[0] += r[0], v[1] += r[1], v[2] += r[2], v[3] += r[3];
     Out* y = static_cast<Out*>(p.y) + row * p.ldy + col;
-    if (p.vec_out && step == 1 && col + 4 <= p.n) {
+    if (VEC && col + 4 <= p.n) {
         if constexpr (OUT_F32) {
             *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
@@ -136,7 +134,9 @@ __device__ __forceinline__ void store_i8_outputs(const GemmI8Params& p, int64_t 
         if (col + e * step < p.n) y[e * step] = static_cast<Out>(v[e]);
 }
 
-template <int BN, bool OUT_F32>
+// RES: with a residual; VEC: rows of y (and of the residual) take vectors of four.
+// Both at compile time: a launch this short pays for every instruction it fetches.
+template <int BN, bool OUT_F32, bool RES, bool VEC>
 __global__ void __launch_bounds__(256)
     gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                         const GemmI8Params p) {
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(256)
     // the four columns of a thread: neighbours where rows take vectors of four, else
     // LANES apart, so that single values of a row are still written side by side
     const int my = threadIdx.x % LANES;
-    const int cstep = p.vec_out ? 1 : LANES;
-    const int my_col = p.vec_out ? 4 * my : my;
+    constexpr int cstep = VEC ? 1 : LANES;
+    const int my_col = VEC ? 4 * my : my;
     const int col = n0 + my_col;
     float ws[4], b[4];
 #pragma unroll
@@ -251,6 +251,19 @@ __global__ void __launch_bounds__(256)
         if (p.bias != nullptr && c < p.n)
             b[e] = p.bias_f32 ? static_cast<const float*>(p.bias)[c] : __half2float(static_cast<const __half*>(p.bias)[c]);
     }
+    // rows of a thread at once; with a residual eight (with 64 columns all it has), whose
+    // values come early: y may be the residual, so none of them may wait behind a store
+    constexpr int BATCH = RES ? 8 : 4;
+    const int r_lo = split * rows / S, r_hi = (split + 1) * rows / S;  // this CTA's share of the rows
+    const int r_first = r_lo + threadIdx.x / LANES;
+    float res[BATCH][4];
+    auto load_residuals = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (r0 + i * STEP < r_hi && col < p.n)
+                load_i8_residual<OUT_F32, VEC>(p, m0 + r0 + i * STEP, col, cstep, res[i]);
+    };
+    if constexpr (RES) load_residuals(r_first);
     if (threadIdx.x < 128) s_xs[threadIdx.x] = static_cast<int>(threadIdx.x) < rows ? __ldg(p.x_scale + m0 + threadIdx.x) : 0.0f;
     __syncwarp();
     volatile int no_abort = 0;
@@ -285,19 +298,15 @@ __global__ void __launch_bounds__(256)
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem_base, BN);
     // ---------------------------------------------------------------- scales, bias, activation, residual
-    const int r_lo = split * rows / S, r_hi = (split + 1) * rows / S;
     if (ok && col < p.n) {
-        for (int r0 = r_lo + threadIdx.x / LANES; r0 < r_hi; r0 += 4 * STEP) {
-            float res[4][4];
+        for (int r0 = r_first; r0 < r_hi; r0 += BATCH * STEP) {
+            if (RES && r0 != r_first) load_residuals(r0);
+            int a[BATCH][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r0 + i * STEP < r_hi) load_i8_residual<OUT_F32>(p, m0 + r0 + i * STEP, col, cstep, res[i]);
-            int a[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < BATCH; ++i) {
                 const int32_t* at = staged + (r0 + i * STEP) * C::ROW + my_col;
                 if (r0 + i * STEP >= r_hi) continue;
-                if (p.vec_out) {
+                if constexpr (VEC) {
                     const int4 t = *reinterpret_cast<const int4*>(at);
                     a[i][0] = t.x, a[i][1] = t.y, a[i][2] = t.z, a[i][3] = t.w;
                 } else {
@@ -308,12 +317,12 @@ __global__ void __launch_bounds__(256)
             for (int o = 1; o < S; ++o) {
                 const uint32_t from = static_cast<uint32_t>(split + o < S ? split + o : split + o - S);
                 const uint32_t base = mapa_shared(smem_u32(staged + my_col), from);
-                int t[4][4];
+                int t[BATCH][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < BATCH; ++i) {
                     const uint32_t at = base + (r0 + i * STEP) * C::ROW * 4;
                     if (r0 + i * STEP >= r_hi) continue;
-                    if (p.vec_out) {
+                    if constexpr (VEC) {
                         const int4 u = ld_shared_cluster_v4(at);
                         t[i][0] = u.x, t[i][1] = u.y, t[i][2] = u.z, t[i][3] = u.w;
                     } else {
@@ -322,20 +331,20 @@ __global__ void __launch_bounds__(256)
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < BATCH; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (r0 + i * STEP < r_hi) a[i][e] += t[i][e];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < BATCH; ++i) {
                 const int r = r0 + i * STEP;
                 if (r >= r_hi) break;
                 const float xs = s_xs[r];
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = fmaf(__int2float_rn(a[i][e]) * ws[e], xs, b[e]);
-                store_i8_outputs<OUT_F32>(p, m0 + r, col, cstep, v, res[i]);
+                store_i8_outputs<OUT_F32, RES, VEC>(p, m0 + r, col, cstep, v, res[i]);
             }
         }
     }

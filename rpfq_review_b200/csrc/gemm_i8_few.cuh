@@ -178,9 +178,13 @@ __global__ void __launch_bounds__(kFewThreads) gemm_i8_few_kernel(const GemmI8Fe
     if (p.g.bias != nullptr)
         b = p.g.bias_f32 ? static_cast<const float*>(p.g.bias)[col] : __half2float(static_cast<const __half*>(p.g.bias)[col]);
     float v[4] = {fmaf(__int2float_rn(mine) * p.g.w_scale[col], s_scale[r], b), 0.0f, 0.0f, 0.0f};
-    float res[4];
-    load_i8_residual<OUT_F32>(p.g, r, col, p.g.n, res);  // one column: the others lie past n
-    store_i8_outputs<OUT_F32>(p.g, r, col, p.g.n, v, res);
+    // one column: the others lie past n
+    float res[4] = {};
+    if (p.g.residual != nullptr) load_i8_residual<OUT_F32, false>(p.g, r, col, p.g.n, res);
+    if (p.g.residual != nullptr)
+        store_i8_outputs<OUT_F32, true, false>(p.g, r, col, p.g.n, v, res);
+    else
+        store_i8_outputs<OUT_F32, false, false>(p.g, r, col, p.g.n, v, res);
 }
 
 }  // namespace rpfq

@@ -844,7 +844,7 @@ int quantize_rows(const char* who, const void* x, bool f32, int64_t ldx, int8_t*
 // ---------------------------------------------------------------- int8 product
 constexpr int32_t kGemmI8MaxK = 131071;  // 128 * 128 * k < 2^31
 
-template <int BN, bool OUT_F32>
+template <int BN, bool OUT_F32, bool RES, bool VEC>
 int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t stream) {
     using C = GemmI8TileCfg<BN>;
     static std::once_flag once[kMaxDevices];
@@ -852,7 +852,7 @@ int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t 
     int dev = 0;
     RPFQ_CUDA(cudaGetDevice(&dev));
     std::call_once(once[dev], [dev]() {
-        attr_status[dev] = cudaFuncSetAttribute(gemm_i8_tile_kernel<BN, OUT_F32>,
+        attr_status[dev] = cudaFuncSetAttribute(gemm_i8_tile_kernel<BN, OUT_F32, RES, VEC>,
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     });
     RPFQ_CUDA(attr_status[dev]);
@@ -862,9 +862,18 @@ int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t 
     if (rc) return rc;
     const int64_t tiles = ((a->m + 127) / 128) * ((a->n + BN - 1) / BN);
     if (tiles * p.splits > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
-    RPFQ_CUDA(launch_kernel(gemm_i8_tile_kernel<BN, OUT_F32>, dim3(static_cast<unsigned>(tiles * p.splits)),
-                            dim3(C::THREADS), C::SMEM_BYTES, stream, p.splits, tx, tw, p));
+    RPFQ_CUDA((launch_kernel(gemm_i8_tile_kernel<BN, OUT_F32, RES, VEC>, dim3(static_cast<unsigned>(tiles * p.splits)),
+                             dim3(C::THREADS), C::SMEM_BYTES, stream, p.splits, tx, tw, p)));
     return RPFQ_OK;
+}
+
+template <int BN, bool OUT_F32>
+int launch_i8_tile(const RpfqGemmI8Args* a, const GemmI8Params& p, cudaStream_t stream) {
+    if (a->residual)
+        return p.vec_out ? launch_i8_tile<BN, OUT_F32, true, true>(a, p, stream)
+                         : launch_i8_tile<BN, OUT_F32, true, false>(a, p, stream);
+    return p.vec_out ? launch_i8_tile<BN, OUT_F32, false, true>(a, p, stream)
+                     : launch_i8_tile<BN, OUT_F32, false, false>(a, p, stream);
 }
 
 // Co-resident CTA pairs of the int8 pair kernel (queried once per device and variant; 0 on error).
@@ -987,8 +996,8 @@ int i8_max_clusters(int splits, DeviceState* st) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
     std::call_once(once[dev][splits], [dev, splits, st]() {
         using C = GemmI8TileCfg<BN>;
-        if (cudaFuncSetAttribute(gemm_i8_tile_kernel<BN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 C::SMEM_BYTES) != cudaSuccess) {
+        const auto kernel = gemm_i8_tile_kernel<BN, false, false, true>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) != cudaSuccess) {
             cudaGetLastError();
             return;
         }
@@ -1004,7 +1013,7 @@ int i8_max_clusters(int splits, DeviceState* st) {
         q.attrs = qa;
         q.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_tile_kernel<BN, false>, &q) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &q) != cudaSuccess) {
             cudaGetLastError();
             return;
         }
@@ -1020,19 +1029,22 @@ struct I8Plan {
 
 // Tile width and k parts of one call, by the least estimated time (us, fitted to
 // CUDA-graph timings on B200 over m = 16..4000, n = 300..4096, k = 390..4096; kb:
-// k-blocks of 128). A wave of the tile kernel costs 2.3, 0.010 (64 columns) or 0.021
-// (128) per live row of its epilogue and 0.15 per k-block of a CTA (an SM streams the
-// operands alone); a split adds 0.7 + 0.0016 rows S for the cluster's exchange. CTA pairs
-// start at 3.9 + 0.28 kb, and a further wave costs max(0.28 kb, 2) + 0.3, its tiles cut
-// when it is at most half full. Measured (us, 64 / 128 wide, best S / pairs): 197 x
-// 1024 x 1024 (m, n, k) 4.6 / 5.8 / 6.1; 64 x 1024 x 4096 4.9 / 5.5 / 12.2; 1576 x 1024
-// x 4096 16.3 / 10.5 / 12.9; 1576 x 768 x 768 8.0 / 5.8 / 5.7; 3152 x 768 x 768 12.8 /
-// 10.0 / 6.1. More than four parts were never the best.
+// k-blocks of 128). A wave of the tile kernel costs 2.3, 0.006 (64 columns) or 0.015
+// (128) per live row of its epilogue and 0.14 per k-block of a CTA (an SM streams the
+// operands alone), 0.29 where rows of codes are no multiple of 128 bytes (a row of a
+// block then lies in two lines); a split adds 0.5 + 0.003 rows S for the cluster's
+// exchange. CTA pairs start at 3.9 + 0.28 (0.47) kb, and a further wave costs max(that
+// per k-block, 2) + 0.3, its tiles cut when it is at most half full. Measured (us, 64 /
+// 128 wide, best S / pairs): 197 x 1024 x 1024 (m, n, k) 4.1 / 5.4 / 6.1; 64 x 1024 x
+// 4096 4.8 / 5.5 / 12.2; 1000 x 300 x 2000 6.8 / 7.7 / 11.4; 1576 x 1024 x 4096 15.2 /
+// 9.8 / 12.9; 1576 x 768 x 768 7.3 / 5.1 / 5.8; 3152 x 768 x 768 11.5 / 9.2 / 6.2. More
+// than four parts were never the best.
 I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
     const int kb = (a->k + 127) / 128;
     if (a->block_n == 256) return {256, 1};
     const int forced = a->split_k ? std::min(a->split_k, kb) : 0;
     const double rows = static_cast<double>(std::min<int64_t>(a->m, 128));
+    const bool lines = a->ldx % 128 == 0 && a->ldw % 128 == 0;
     const int64_t row_tiles = (a->m + 127) / 128;
     I8Plan best = {a->block_n ? a->block_n : 128, forced ? forced : 1};
     double cost = -1.0;
@@ -1045,8 +1057,8 @@ I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
             if (fit <= 0) continue;
             const int64_t tiles = row_tiles * ((a->n + bn - 1) / bn);
             const double waves = static_cast<double>((tiles + fit - 1) / fit);
-            const double c = waves * (2.3 + (bn == 64 ? 0.010 : 0.021) * rows + 0.15 * ((kb + s - 1) / s)) +
-                             (s > 1 ? 0.7 + 0.0016 * rows * s : 0.0);
+            const double c = waves * (2.3 + (bn == 64 ? 0.006 : 0.015) * rows + (lines ? 0.14 : 0.29) * ((kb + s - 1) / s)) +
+                             (s > 1 ? 0.5 + 0.003 * rows * s : 0.0);
             if (cost < 0 || c < cost) {
                 cost = c;
                 best = {bn, s};
@@ -1061,7 +1073,8 @@ I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
     const double more = pair_tiles <= units ? 0.0
                                             : static_cast<double>(pair_tiles / units - 1) +
                                                   (rest == 0 ? 0.0 : (2 * rest <= units ? 0.5 : 1.0));
-    const double pairs = 3.9 + 0.28 * kb + more * (std::max(0.28 * kb, 2.0) + 0.3);
+    const double main = (lines ? 0.28 : 0.47) * kb;
+    const double pairs = 3.9 + main + more * (std::max(main, 2.0) + 0.3);
     if (cost < 0 || pairs < cost) best = {256, 1};
     return best;
 }

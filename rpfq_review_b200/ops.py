@@ -511,15 +511,17 @@ def act_quant(x: torch.Tensor, num_bits: int, out: torch.Tensor | None = None) -
 GEMM_INT8_MAX_K = 131071  # 128 * 128 * k < 2^31: the int32 sums cannot overflow
 
 
-def _forward_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+def _tensors(name: str, index: int, differentiable, others) -> None:
+    """Every tensor (None: not given) is on cuda:index, and no gradient is asked for
+    through the first ones: these operators have no autograd."""
+    grad = torch.is_grad_enabled()
+    for t in differentiable:
+        if t is not None:
+            if t.get_device() != index:
+                raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
+            if grad and t.requires_grad:
                 raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
-
-
-def _same_device(name: str, index: int, *tensors) -> None:
-    for t in tensors:
+    for t in others:
         if t is not None and t.get_device() != index:
             raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
 
@@ -575,22 +577,26 @@ def quantize_rows(x: torch.Tensor):
     infinity gets codes of zero and a scale of NaN. The tokens of an activation
     matrix, or the output channels of a weight ``[n, k]``."""
     f32 = _float_type(x, "x")
-    _forward_only("quantize_rows", x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(x.shape)}")
-    k = x.shape[-1]
+    index = x.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return quantize_rows(x)
+    _tensors("quantize_rows", index, (x,), ())
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(shape)}")
+    k, lead = shape[-1], shape[:-1]
     x2, m, ldx = _matrix(x, k, "x")
     ld = (k + 15) // 16 * 16
-    q = torch.empty((m, ld), dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().rpfq_quantize_rows_sm100(x2.data_ptr(), int(f32), ldx, q.data_ptr(), ld,
-                                                       scale.data_ptr(), m, k, _stream(x.device)),
-                   "rpfq_quantize_rows_sm100")
-    if m:
+    q = x.new_empty((*lead, ld), dtype=torch.int8)
+    scale = x.new_empty(lead, dtype=torch.float32)
+    rc = _lib.lib().rpfq_quantize_rows_sm100(x2.data_ptr(), int(f32), ldx, q.data_ptr(), ld, scale.data_ptr(), m, k,
+                                             torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, "rpfq_quantize_rows_sm100")
+    if _timer is not None and m:
         _count_launch()
-    codes = q.view(*x.shape[:-1], ld)
-    return (codes if ld == k else codes[..., :k]), scale
+    return (q if ld == k else q[..., :k]), scale
 
 
 def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int, ldx: int, x_scale, x_flag: int,
@@ -601,19 +607,14 @@ def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int,
         with torch.cuda.device(index):
             return _gemm_int8(name, index, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
                               out_dtype, block_n, split_k)
-    _forward_only(name, w_scale, residual)
-    _same_device(name, index, w, w_scale, bias, residual, out)
+    _tensors(name, index, (x, w_scale, residual), (w, bias, out))
     n, k = w.shape
     if w_scale.dtype is not torch.float32 or w_scale.numel() != n:
         raise ValueError(f"{name}: w_scale must hold {n} float32 values, got {w_scale.numel()} of {w_scale.dtype}")
-    if activation not in _ACT:
+    act = _ACT.get(activation)
+    if act is None:
         raise ValueError(f"{name}: unknown activation {activation!r}")
-    bias_ptr = None
-    if bias is not None:
-        if bias.numel() != n:
-            raise ValueError(f"{name}: bias must hold {n} values, got {bias.numel()}")
-        bias = bias.contiguous()
-        bias_ptr = bias.data_ptr()
+    flags, bias_ptr, r_ptr, ldr = x_flag, None, None, 0
     w2, _, ldw = _code_rows(w, k, "w")
     w_scale = w_scale.contiguous()
     if out is None:
@@ -621,25 +622,45 @@ def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int,
         ldy = n
     else:
         y2, rows, ldy = _matrix(out, n, "out")
+        out_dtype = out.dtype
         if y2.data_ptr() != out.data_ptr() or rows != m:
             raise ValueError(f"{name}: out must be a row-major view of {m} rows with unit column stride")
-    r2, ldr, r_ptr = None, 0, None
+    if out_dtype is torch.float32:
+        flags |= _lib.GEMM_OUT_F32
+    elif out_dtype is not torch.float16:
+        raise ValueError(f"{name}: out must be float16 or float32, got {out_dtype}")
+    if bias is not None:
+        if bias.numel() != n:
+            raise ValueError(f"{name}: bias must hold {n} values, got {bias.numel()}")
+        if bias.dtype is torch.float32:
+            flags |= _lib.GEMM_BIAS_F32
+        elif bias.dtype is not torch.float16:
+            raise ValueError(f"{name}: bias must be float16 or float32, got {bias.dtype}")
+        bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
     if residual is not None:
         r2, rows, ldr = _matrix(residual, n, "residual")
         if rows != m:
             raise ValueError(f"{name}: residual rows do not match x")
+        if r2.dtype is torch.float32:
+            flags |= _lib.GEMM_RESIDUAL_F32
+        elif r2.dtype is not torch.float16:
+            raise ValueError(f"{name}: residual must be float16 or float32, got {r2.dtype}")
         r_ptr = r2.data_ptr()
     L = _lib.lib()
-    scratch, need = None, 0
+    scratch, scratch_ptr, need = None, None, 0
     if x_flag:
+        # a few rows are quantized inside the launch; the library says which
         need = m * ((k + 15) // 16 * 16 + 4) if block_n or split_k else L.rpfq_gemm_i8_scratch_bytes(m, k)
         if need:
             scratch = x.new_empty(need, dtype=torch.uint8)
+            scratch_ptr = scratch.data_ptr()
     a = _lib.RpfqGemmI8Args(x2.data_ptr(), ldx, x_scale, w2.data_ptr(), ldw, w_scale.data_ptr(), bias_ptr, r_ptr, ldr,
-                            out.data_ptr(), ldy, m, n, k, _ACT[activation], x_flag | _flags(out, r2, bias),
-                            block_n, split_k, _p(scratch), need)
-    _lib.check(L.rpfq_gemm_i8_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index)), "rpfq_gemm_i8_sm100")
-    if m:
+                            out.data_ptr(), ldy, m, n, k, act, flags, block_n, split_k, scratch_ptr, need)
+    rc = L.rpfq_gemm_i8_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, "rpfq_gemm_i8_sm100")
+    if _timer is not None and m:
         _count_launch(2 if need else 1)
     return out
 
@@ -667,8 +688,7 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     _require(x, "x", torch.int8)
     _check_codes(name, w)
     index = x.get_device()
-    _forward_only(name, x_scale)
-    _same_device(name, index, x_scale)
+    _tensors(name, index, (x_scale,), ())
     x2, m, ldx = _code_rows(x, w.shape[1], "x")
     if x_scale.dtype is not torch.float32 or x_scale.numel() != m:
         raise ValueError(f"{name}: x_scale must hold one float32 value per row ({m}), got {x_scale.numel()} of "
@@ -688,7 +708,6 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     name = "linear_int8"
     x_flag = _lib.GEMM_X_F32 if _float_type(x, "x") else _lib.GEMM_X_F16
     _check_codes(name, w)
-    _forward_only(name, x)
     x2, m, ldx = _matrix(x, w.shape[1], "x")
     return _gemm_int8(name, x.get_device(), x, x2, m, ldx, None, x_flag, w, w_scale, bias, residual, activation, out,
                       out_dtype, block_n, split_k)
@@ -767,55 +786,55 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     of the output to the gradient of x."""
     name = "rotary"
     f32 = _float_type(x, "x")
-    _forward_only(name, x)
-    if x.dim() not in (3, 4):
+    index = x.get_device()
+    _tensors(name, index, (x,), (positions, inv_freq, out))
+    four = x.dim() == 4
+    if not four and x.dim() != 3:
         raise ValueError(f"{name}: x must be [L, H, D] or [B, L, H, D], got {tuple(x.shape)}")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"{name}: layout must be 'half' or 'interleaved', got {layout!r}")
     if axes not in (1, 2):
         raise ValueError(f"{name}: axes must be 1 or 2, got {axes}")
-    _require(inv_freq, "inv_freq", torch.float64)
-    L, H, D = x.shape[-3:]
-    B = x.shape[0] if x.dim() == 4 else 1
+    if inv_freq.dtype is not torch.float64:
+        raise ValueError(f"{name}: inv_freq must be float64, got {inv_freq.dtype}")
+    B, L, H, D = x.shape if four else (1, *x.shape)
     pairs = inv_freq.numel()
     if pairs == 0 or 2 * pairs > D or pairs % axes:
         raise ValueError(f"{name}: inv_freq must hold 1..{D // 2} values, a multiple of axes, got {pairs}")
-    if not positions.is_cuda or positions.dtype not in _POSITION:
-        raise ValueError(f"{name}: positions must be an int32, int64, float32 or float64 CUDA tensor")
+    position_type = _POSITION.get(positions.dtype)
+    if position_type is None:
+        raise ValueError(f"{name}: positions must be int32, int64, float32 or float64, got {positions.dtype}")
     tail = (axes,) if axes > 1 else ()
-    shape = tuple(positions.shape)
+    shape = positions.shape
     if shape == (L, *tail):
         per_sequence = 0
-    elif x.dim() == 4 and shape == (B, L, *tail):
+    elif four and shape == (B, L, *tail):
         per_sequence = L * axes
     else:
-        raise ValueError(f"{name}: positions must be {(L, *tail)} or {(B, L, *tail)}, got {shape}")
+        raise ValueError(f"{name}: positions must be {(L, *tail)} or {(B, L, *tail)}, got {tuple(shape)}")
     if x.stride(-1) != 1 and D > 1:
         if out is x:
             raise ValueError(f"{name}: in place, a head must have unit stride")
         x = x.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError(f"{name}: out must be {tuple(x.shape)} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
     elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or (D > 1 and out.stride(-1) != 1):
         raise ValueError(f"{name}: out must not be expanded and must have unit stride inside a head")
-    index = x.get_device()
-    _same_device(name, index, positions, inv_freq, out)
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     xs, ys = x.stride(), out.stride()
-    four = len(xs) == 4
     a = _lib.RpfqRotaryArgs(x.data_ptr(), xs[0] if four else 0, xs[-3], xs[-2], out.data_ptr(), ys[0] if four else 0,
                             ys[-3], ys[-2], positions.data_ptr(), per_sequence, inv_freq.data_ptr(), B, L, H, D,
-                            pairs, axes, _POSITION[positions.dtype], f32, layout == "interleaved", bool(transpose),
-                            magnitude)
+                            pairs, axes, position_type, f32, layout == "interleaved", bool(transpose), magnitude)
     if torch.cuda.current_device() == index:
         rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
-    _lib.check(rc, "rpfq_rotary_sm100")
-    if x.numel():
+    if rc:
+        _lib.check(rc, "rpfq_rotary_sm100")
+    if _timer is not None and x.numel():
         _count_launch()
     return out
 

@@ -911,6 +911,13 @@ int i8_pair_units(DeviceState* st) {
     return units[dev];
 }
 
+// Rows of n values at stride ld that the pair kernel moves by TMA. n in whole 16 bytes:
+// a TMA store of fewer writes to the end of the last 16 all the same, into what lies
+// behind a row of a wider buffer.
+bool i8_tma_rows(const void* base, int64_t ld, int64_t n, int64_t esize) {
+    return aligned16(base) && ld * esize % 16 == 0 && n * esize % 16 == 0;
+}
+
 template <bool OUT_F32, bool RES, int EW>
 int launch_i8_pair(const RpfqGemmI8Args* a, GemmI8Params p, DeviceState* st, cudaStream_t stream) {
     const int units = i8_pair_units<OUT_F32, RES, EW>(st);
@@ -922,8 +929,8 @@ int launch_i8_pair(const RpfqGemmI8Args* a, GemmI8Params p, DeviceState* st, cud
     if (tiles > 0x7fffffff - units) return fail(RPFQ_ERR_UNSUPPORTED, "rpfq_gemm_i8_sm100: too many tiles");
     p.pieces = narrow_pieces(tiles, units);
     p.tail_tiles = p.pieces ? static_cast<int32_t>(tiles % units) : 0;
-    p.vec_out = aligned16(a->y) && a->ldy * ESZ % 16 == 0;
-    p.vec_res = a->residual && aligned16(a->residual) && a->ldr * ESZ % 16 == 0;
+    p.vec_out = i8_tma_rows(a->y, a->ldy, a->n, ESZ);
+    p.vec_res = a->residual && i8_tma_rows(a->residual, a->ldr, a->n, ESZ);
     CUtensorMap tx, tw, twp, ty, tr;
     int rc = make_tmap_i8(&tx, a->x, a->m, a->k, a->ldx, C::BM);
     if (!rc) rc = make_tmap_i8(&tw, a->w, a->n, a->k, a->ldw, C::BN / 2);
@@ -1197,7 +1204,7 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
         // stores (20000 x 1001 x 700 fp16 33 / 29, fp32 41 / 32), fp16 rows of a short main
         // loop (50432 x 1152 x 384 36 / 31; x 640 38.9 / 38.3); else the ring's sixth stage
         // is worth more (50432 x 2304 x 1024 fp32 114 / 121, 3152 x 768 x 768 6.2 / 6.8)
-        const bool tma_out = aligned16(a->y) && a->ldy * static_cast<int64_t>(esize) % 16 == 0;
+        const bool tma_out = i8_tma_rows(a->y, a->ldy, a->n, esize);
         if (p.activation == RPFQ_ACT_GELU || !tma_out || (!f32 && a->k <= 512))
             return f32 ? launch_i8_pair<true, false, 16>(a, p, st, stream) : launch_i8_pair<false, false, 16>(a, p, st, stream);
         return f32 ? launch_i8_pair<true, false, 8>(a, p, st, stream) : launch_i8_pair<false, false, 8>(a, p, st, stream);

@@ -242,6 +242,35 @@ def test_gemm_int8_strides(cuda, m, n, k, out_dtype):
     assert all(torch.equal(row[i], row[0]) for i in range(9))
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(4, 3, 15), (31, 63, 130), (300, 255, 63), (513, 1001, 300)])
+def test_gemm_int8_inside_wider_rows(cuda, m, n, k, out_dtype):
+    """Operands, residual and output as columns of wider rows on the 16-byte grid, n and
+    k off it: what lies beside them is neither read nor written, by any schedule."""
+    from rpfq_review_b200 import ops
+    xq, xs, wq, ws = _operands(cuda, m, n, k, seed=19)
+    g = torch.Generator().manual_seed(19)
+    residual = torch.randn(m, n, generator=g).to(out_dtype)
+    ref = _product_ref(xq, xs, wq, ws, None, "none", None, out_dtype)
+    ref_res = _product_ref(xq, xs, wq, ws, None, "none", residual, out_dtype)
+
+    def inside(t, step, beside):
+        buf = torch.full((t.shape[0] + 1, -(-t.shape[1] // step) * step + 2 * step), beside, dtype=t.dtype, device=cuda)
+        view = buf[:-1, step:step + t.shape[1]]
+        view.copy_(t)
+        return view
+
+    xv, wv = inside(xq, 16, 113), inside(wq, 16, 127)
+    rv = inside(residual.to(cuda), 16, float("nan"))
+    for block_n in (0, 64, 128, 256):
+        for res, want in ((None, ref), (rv, ref_res)):
+            out = inside(torch.zeros(m, n, dtype=out_dtype, device=cuda), 16, 7.0)
+            ops.gemm_int8(xv, xs, wv, ws, residual=res, out=out, block_n=block_n)
+            _check(out, want)
+            out.fill_(7.0)
+            assert (out._base == 7.0).all(), f"written beside the output with block_n={block_n}"
+
+
 def test_gemm_int8_nan_scale_stays_in_its_row(cuda):
     from rpfq_review_b200 import ops
     for m in (4, 140, 1000):

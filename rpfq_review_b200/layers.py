@@ -22,6 +22,19 @@ from . import ops
 from .packing import AXIAL_STAGES, BLOCK_SIZE, SUPPORTED_QUANT_METHODS, PackedLayer, pack_linear, round_up
 
 
+def _made_from(tensors):
+    """A record of the tensors that something kept was made from, for :func:`_unchanged`. It holds
+    them and an alias of their memory, so neither they nor their addresses can come back with
+    other values while the record lives."""
+    return [(t, t._version, t.data_ptr(), t.detach()) for t in tensors]
+
+
+def _unchanged(record, tensors) -> bool:
+    """Whether ``tensors`` are those of the record, neither written nor given other memory since."""
+    return record is not None and all(t is s and t._version == version and t.data_ptr() == address
+                                      for t, (s, version, address, _) in zip(tensors, record))
+
+
 class PhasePlane(nn.Module):
     """Buffers of one residual stage: ``codes``, ``gamma_real``, ``gamma_imag``."""
 
@@ -86,7 +99,7 @@ class PackedPhaseLinear(nn.Module):
         # compute="int8": the coefficients as int8 codes [N, K] and fp32 scales [N]
         self.register_buffer("codes8", None, persistent=False)
         self.register_buffer("scale8", None, persistent=False)
-        self._planes8 = None  # the planes (and their versions) that codes8 comes from
+        self._planes8 = None  # record of the planes that codes8 comes from
         self._bias32 = None  # (version, fp32 copy of bias) for the epilogue
 
     # -- construction ---------------------------------------------------------
@@ -135,9 +148,20 @@ class PackedPhaseLinear(nn.Module):
             self._bias32 = (key, self.bias.float())
         return self._bias32[1]
 
-    def _planes_key(self):
-        return tuple((t.data_ptr(), t._version) for tag in ("u", "w") for s in range(self.stages)
-                     for t in getattr(self, f"{tag}_s{s}")._buffers.values())
+    def _plane_tensors(self):
+        return [t for tag in ("u", "w") for s in range(self.stages)
+                for t in getattr(self, f"{tag}_s{s}")._buffers.values()]
+
+    def _apply(self, *args, **kwargs):
+        super()._apply(*args, **kwargs)
+        if self._planes8 is not None and not (_unchanged(self._planes8, self._plane_tensors())
+                                              and self.scale8.dtype == torch.float32):
+            # the planes were moved, or the scales cast: nothing made from them is kept, nor the old planes
+            self._planes8 = self.codes8 = self.scale8 = None
+        return self
+
+    def __getstate__(self):  # a copy makes its own codes
+        return {**self.__dict__, "_planes8": None}
 
     @property
     def _fused_decode_ok(self) -> bool:
@@ -159,9 +183,9 @@ class PackedPhaseLinear(nn.Module):
         ``compute="int8"`` the decoded rows are quantized and only their codes
         and scales are kept; returns the codes."""
         if self.compute == "int8":
-            key = self._planes_key()
+            record = _made_from(self._plane_tensors())
             self.codes8, self.scale8 = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
-            self._planes8 = key
+            self._planes8 = record
             return self.codes8
         self.dense = self._decode_dense()
         return self.dense
@@ -181,7 +205,7 @@ class PackedPhaseLinear(nn.Module):
                                                            else torch.float16)
         if self.compute == "int8":
             # again after the planes were loaded, written or moved, or the scales cast with the module
-            if self.codes8 is None or self._planes8 != self._planes_key() or self.scale8.dtype != torch.float32:
+            if not _unchanged(self._planes8, self._plane_tensors()):
                 self.prepack()
             xf = x if x.dtype in (torch.float16, torch.float32) else x.to(torch.float16)
             return ops.linear_int8(xf, self.codes8, self.scale8, self._bias_f32(), residual, self.activation, out,

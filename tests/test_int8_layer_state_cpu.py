@@ -1,0 +1,90 @@
+"""What an 8-bit layer keeps between calls, on the CPU: the decoder, the row quantizer and the
+product are stand-ins on CPU tensors (the layer's own bookkeeping is the tested code)."""
+
+import numpy as np
+import pytest
+import torch
+
+from rpfq_review_b200 import PackedPhaseLinear, ops
+from rpfq_review_b200.packing import random_packed
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Stand-ins: the "dense matrix" is the first plane's codes as fp32, its "codes" their low
+    seven bits, and the product returns the codes, scales and bias that the layer passes."""
+    made = []
+
+    def prepack(packed, rounding="rne"):
+        made.append(1)
+        return packed.planes["u_s0"][0].float()
+
+    monkeypatch.setattr(ops, "prepack", prepack)
+    monkeypatch.setattr(ops, "quantize_rows", lambda w: ((w % 128).to(torch.int8), w.amax(1).float()))
+    monkeypatch.setattr(ops, "linear_int8", lambda x, w, w_scale, bias, *more: (w.clone(), w_scale.clone(), bias.clone()))
+    return made
+
+
+def _layer(seed=0, **kw):
+    return PackedPhaseLinear.from_packed(random_packed(8, 8, seed=seed), compute="int8", **kw)
+
+
+def _run(layer):
+    return layer(torch.zeros(1, layer.in_features))
+
+
+def _same(got, layer):
+    w = layer.u_s0.codes.float()
+    return torch.equal(got[0], (w % 128).to(torch.int8)) and torch.equal(got[1], w.amax(1))
+
+
+class Pool:
+    """An allocator that hands the same addresses out again: a tensor moved to it lands where the
+    tensor of that name landed before (its memory there is taken to be free)."""
+
+    def __init__(self):
+        self.memory = {}
+
+    def move(self, module):
+        for name, plane in module.named_modules():
+            for key, t in list(plane._buffers.items()):
+                if t is None:
+                    continue
+                at = self.memory.setdefault((name, key), np.empty(t.numel() * t.element_size() + 64, np.uint8))
+                new = torch.from_numpy(at[: t.numel() * t.element_size()]).view(t.dtype).view(t.shape)
+                at[: t.numel() * t.element_size()] = t.detach().contiguous().view(-1).view(torch.uint8).numpy()
+                plane._buffers[key] = new
+
+
+def test_codes_follow_planes_that_move_over_the_same_addresses(calls):
+    """Off, loaded, back on, run, twice: the second time the planes lie where they lay, in new
+    tensors of the same version."""
+    layer, pool = _layer(), Pool()
+    for seed in (1, 2, 3):
+        other = _layer(seed)
+        for name, t in layer.named_buffers():
+            if name.endswith(("codes", "gamma_real", "gamma_imag")):
+                t.copy_(dict(other.named_buffers())[name])
+        pool.move(layer)
+        assert _same(_run(layer), layer), f"codes of older planes with seed {seed}"
+        before = len(calls)
+        assert _same(_run(layer), layer)
+        assert len(calls) == before, "unchanged planes are not decoded again"
+
+
+def test_codes_follow_writes_casts_and_assignments(calls):
+    layer = _layer()
+    _run(layer)
+    layer.u_s0.codes.add_(1)
+    assert _same(_run(layer), layer)
+    layer.u_s0.codes = layer.u_s0.codes.clone().add_(3)
+    assert _same(_run(layer), layer)
+    layer.u_s0.codes.data = layer.u_s0.codes.clone().add_(5)
+    assert _same(_run(layer), layer)
+    layer.load_state_dict(_layer(4).state_dict())
+    assert _same(_run(layer), layer)
+    layer.load_state_dict(_layer(5).state_dict(), assign=True)
+    assert _same(_run(layer), layer)
+    layer.half()
+    got = _run(layer)
+    assert _same(got, layer) and got[1].dtype == torch.float32

@@ -31,8 +31,12 @@ def _made_from(tensors):
 
 def _unchanged(record, tensors) -> bool:
     """Whether ``tensors`` are those of the record, neither written nor given other memory since."""
-    return record is not None and all(t is s and t._version == version and t.data_ptr() == address
-                                      for t, (s, version, address, _) in zip(tensors, record))
+    if record is None:
+        return False
+    for t, (s, version, address, _) in zip(tensors, record):
+        if t is not s or t._version != version or t.data_ptr() != address:
+            return False
+    return True
 
 
 class PhasePlane(nn.Module):
@@ -100,7 +104,7 @@ class PackedPhaseLinear(nn.Module):
         self.register_buffer("codes8", None, persistent=False)
         self.register_buffer("scale8", None, persistent=False)
         self._planes8 = None  # record of the planes that codes8 comes from
-        self._bias32 = None  # (version, fp32 copy of bias) for the epilogue
+        self._bias32 = None  # (record of bias, its fp32 copy) for the epilogue
 
     # -- construction ---------------------------------------------------------
     @classmethod
@@ -143,9 +147,8 @@ class PackedPhaseLinear(nn.Module):
     def _bias_f32(self) -> torch.Tensor:
         """The fp16 bias widened to fp32 once (exact); refreshed when the
         bias tensor changes."""
-        key = (self.bias.data_ptr(), self.bias._version, self.bias.device)
-        if self._bias32 is None or self._bias32[0] != key:
-            self._bias32 = (key, self.bias.float())
+        if self._bias32 is None or not _unchanged(self._bias32[0], (self.bias,)):
+            self._bias32 = (_made_from((self.bias,)), self.bias.float())
         return self._bias32[1]
 
     def _plane_tensors(self):
@@ -158,10 +161,12 @@ class PackedPhaseLinear(nn.Module):
                                               and self.scale8.dtype == torch.float32):
             # the planes were moved, or the scales cast: nothing made from them is kept, nor the old planes
             self._planes8 = self.codes8 = self.scale8 = None
+        if self._bias32 is not None and not _unchanged(self._bias32[0], (self.bias,)):
+            self._bias32 = None
         return self
 
-    def __getstate__(self):  # a copy makes its own codes
-        return {**self.__dict__, "_planes8": None}
+    def __getstate__(self):  # a copy makes its own codes and fp32 bias
+        return {**self.__dict__, "_planes8": None, "_bias32": None}
 
     @property
     def _fused_decode_ok(self) -> bool:

@@ -29,3 +29,18 @@ def test_two_moves_with_other_planes(cuda):
         layer.to(cuda)
         other.bias.copy_(layer.bias)
         assert torch.equal(layer(x), other(x)), seed
+
+
+@pytest.mark.parametrize("compute", ["int8", "fp16"])
+def test_two_moves_with_another_bias(cuda, compute):
+    from rpfq_review_b200 import PackedPhaseLinear
+    from rpfq_review_b200.packing import random_packed
+    layer, x = PackedPhaseLinear.from_packed(random_packed(96, 64, seed=0, device=cuda), compute=compute), _x()
+    layer.bias.zero_()
+    y = layer(x)
+    for step in (1.0, 2.0, 4.0, 8.0):
+        layer.cpu()
+        layer.bias.fill_(step)
+        layer.to(cuda)
+        # y + step in fp32 rounds once more than the epilogue: 2^-24 of values below 256
+        assert (layer(x) - (y + step)).abs().max() <= 2.0 ** -14, step

@@ -88,3 +88,13 @@ def test_codes_follow_writes_casts_and_assignments(calls):
     layer.half()
     got = _run(layer)
     assert _same(got, layer) and got[1].dtype == torch.float32
+
+
+def test_bias_follows_moves_over_the_same_addresses(calls):
+    layer, pool = _layer(), Pool()
+    for step in (1, 2, 3):
+        layer.bias.fill_(step)
+        pool.move(layer)
+        assert (_run(layer)[2] == step).all()
+    layer.bias.fill_(7)
+    assert (_run(layer)[2] == 7).all()

@@ -39,6 +39,12 @@ def _unchanged(record, tensors) -> bool:
     return True
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    """Whether what is made from ``t`` now belongs to a CUDA graph: written when that is replayed,
+    in memory of its own, so not to be kept for other calls."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class PhasePlane(nn.Module):
     """Buffers of one residual stage: ``codes``, ``gamma_real``, ``gamma_imag``."""
 
@@ -147,9 +153,24 @@ class PackedPhaseLinear(nn.Module):
     def _bias_f32(self) -> torch.Tensor:
         """The fp16 bias widened to fp32 once (exact); refreshed when the
         bias tensor changes."""
-        if self._bias32 is None or not _unchanged(self._bias32[0], (self.bias,)):
-            self._bias32 = (_made_from((self.bias,)), self.bias.float())
-        return self._bias32[1]
+        if self._bias32 is not None and _unchanged(self._bias32[0], (self.bias,)):
+            return self._bias32[1]
+        bias = self.bias.float()
+        if not _capturing(self.bias):
+            self._bias32 = (_made_from((self.bias,)), bias)
+        return bias
+
+    def _int8_weight(self):
+        """The coefficients as int8 codes and fp32 scales: made once, and again after the planes
+        were loaded, written or moved, or the scales cast with the module."""
+        planes = self._plane_tensors()
+        if _unchanged(self._planes8, planes):
+            return self.codes8, self.scale8
+        record = _made_from(planes)
+        codes, scale = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
+        if not _capturing(codes):
+            self.codes8, self.scale8, self._planes8 = codes, scale, record
+        return codes, scale
 
     def _plane_tensors(self):
         return [t for tag in ("u", "w") for s in range(self.stages)
@@ -188,10 +209,8 @@ class PackedPhaseLinear(nn.Module):
         ``compute="int8"`` the decoded rows are quantized and only their codes
         and scales are kept; returns the codes."""
         if self.compute == "int8":
-            record = _made_from(self._plane_tensors())
-            self.codes8, self.scale8 = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
-            self._planes8 = record
-            return self.codes8
+            self._planes8 = None
+            return self._int8_weight()[0]
         self.dense = self._decode_dense()
         return self.dense
 
@@ -209,12 +228,8 @@ class PackedPhaseLinear(nn.Module):
             out_dtype = out.dtype if out is not None else (x.dtype if x.dtype in (torch.float16, torch.float32)
                                                            else torch.float16)
         if self.compute == "int8":
-            # again after the planes were loaded, written or moved, or the scales cast with the module
-            if not _unchanged(self._planes8, self._plane_tensors()):
-                self.prepack()
             xf = x if x.dtype in (torch.float16, torch.float32) else x.to(torch.float16)
-            return ops.linear_int8(xf, self.codes8, self.scale8, self._bias_f32(), residual, self.activation, out,
-                                   out_dtype)
+            return ops.linear_int8(xf, *self._int8_weight(), self._bias_f32(), residual, self.activation, out, out_dtype)
         x16 = x if x.dtype == torch.float16 else x.to(torch.float16)
         act_bits = 0 if prequantized else self.act_bits
         if self.vision_quant is not None and not prequantized:

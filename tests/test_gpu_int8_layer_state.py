@@ -44,3 +44,19 @@ def test_two_moves_with_another_bias(cuda, compute):
         layer.to(cuda)
         # y + step in fp32 rounds once more than the epilogue: 2^-24 of values below 256
         assert (layer(x) - (y + step)).abs().max() <= 2.0 ** -14, step
+
+
+def test_first_call_inside_a_capture(cuda):
+    """A layer whose first call is captured: eager calls before the first replay have their own
+    codes and bias, and the replay follows planes loaded after the capture."""
+    layer, x = _layer(1), _x()
+    want = _layer(1)(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x)
+    assert torch.equal(layer(x), want)
+    g.replay()
+    assert torch.equal(y, want)
+    layer.load_state_dict(_layer(2).state_dict())
+    g.replay()
+    assert torch.equal(y, _layer(2)(x)) and torch.equal(layer(x), y)

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from rpfq_review_b200 import PackedPhaseLinear, ops
+from rpfq_review_b200 import PackedPhaseLinear, layers, ops
 from rpfq_review_b200.packing import random_packed
 
 
@@ -98,3 +98,13 @@ def test_bias_follows_moves_over_the_same_addresses(calls):
         assert (_run(layer)[2] == step).all()
     layer.bias.fill_(7)
     assert (_run(layer)[2] == 7).all()
+
+
+def test_nothing_made_inside_a_capture_is_kept(calls, monkeypatch):
+    """What a captured call makes is written when its graph is replayed, into the graph's memory."""
+    layer = _layer()
+    monkeypatch.setattr(layers, "_capturing", lambda t: True)
+    assert _same(_run(layer), layer) and layer.codes8 is None and layer._bias32 is None
+    layer.prepack()
+    assert layer.codes8 is None
+    monkeypatch.undo()

@@ -45,6 +45,25 @@ def _capturing(t: torch.Tensor) -> bool:
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+def _keep(kept, made):
+    """What a module keeps between calls, made again (``kept`` None: for the first time): the tensors
+    ``made``, in the memory of ``kept`` where that fits, since captured graphs may read it. Calls of any
+    stream may be reading ``kept`` and may use the result at once, so the GPU finishes the former
+    before and the copies after. Returns the tensors to keep."""
+    device = made[0].device
+    if kept is not None and all(k.shape == m.shape and k.dtype == m.dtype and k.device == m.device
+                                for k, m in zip(kept, made)):
+        if device.type == "cuda":
+            torch.cuda.synchronize(device)
+        with torch.inference_mode():  # kept may have been made in it
+            for k, m in zip(kept, made):
+                k.copy_(m)
+        made = kept
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+    return made
+
+
 class PhasePlane(nn.Module):
     """Buffers of one residual stage: ``codes``, ``gamma_real``, ``gamma_imag``."""
 
@@ -157,7 +176,9 @@ class PackedPhaseLinear(nn.Module):
             return self._bias32[1]
         bias = self.bias.float()
         if not _capturing(self.bias):
-            self._bias32 = (_made_from((self.bias,)), bias)
+            record = _made_from((self.bias,))
+            (bias,) = _keep(None if self._bias32 is None else self._bias32[1:], (bias,))
+            self._bias32 = (record, bias)
         return bias
 
     def _int8_weight(self):
@@ -169,6 +190,7 @@ class PackedPhaseLinear(nn.Module):
         record = _made_from(planes)
         codes, scale = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
         if not _capturing(codes):
+            codes, scale = _keep(None if self.codes8 is None else (self.codes8, self.scale8), (codes, scale))
             self.codes8, self.scale8, self._planes8 = codes, scale, record
         return codes, scale
 
@@ -207,7 +229,7 @@ class PackedPhaseLinear(nn.Module):
         """Decode the packed planes once (K1). Layers whose real dims are not
         multiples of 8 keep a zero-padded copy ``[N8, K8]`` for the GEMM. With
         ``compute="int8"`` the decoded rows are quantized and only their codes
-        and scales are kept; returns the codes."""
+        and scales are kept (in the same memory when planes change); returns the codes."""
         if self.compute == "int8":
             self._planes8 = None
             return self._int8_weight()[0]

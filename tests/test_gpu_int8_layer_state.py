@@ -60,3 +60,52 @@ def test_first_call_inside_a_capture(cuda):
     layer.load_state_dict(_layer(2).state_dict())
     g.replay()
     assert torch.equal(y, _layer(2)(x)) and torch.equal(layer(x), y)
+
+
+SLEEP = 40_000_000  # clock cycles: about 20 ms, far longer than what runs beside it
+
+
+def test_codes_are_ready_for_every_stream(cuda):
+    """Made behind other work of one stream, used at once by another."""
+    for seed in range(3):
+        layer, x, want = _layer(seed), _x(), _layer(seed)(_x())
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(SLEEP)
+            ya = layer(x)
+        with torch.cuda.stream(b):
+            yb = layer(x)
+        torch.cuda.synchronize()
+        assert torch.equal(ya, want) and torch.equal(yb, want)
+
+
+def test_codes_in_use_are_not_overwritten(cuda):
+    """Planes loaded while a call on another stream still waits to read the old codes."""
+    layer, other, x = _layer(1), _layer(2), _x()
+    old, new = layer(x), other(x)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+        y = layer(x)
+    layer.load_state_dict(other.state_dict())
+    z = layer(x)
+    torch.empty(1 << 24, dtype=torch.uint8, device=cuda).fill_(17)
+    torch.cuda.synchronize()
+    assert torch.equal(y, old) and torch.equal(z, new)
+
+
+def test_graph_reads_the_codes_of_loaded_planes(cuda):
+    """A captured call reads the kept codes: they stay where they are when planes are loaded."""
+    layer, x = _layer(1), _x()
+    layer(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x)
+    for seed in (2, 3):
+        layer.load_state_dict(_layer(seed).state_dict())
+        want = layer(x)
+        noise = [torch.full_like(layer.codes8, 17), torch.full_like(layer.scale8, 3.0), torch.full_like(want[0], 5.0)]
+        g.replay()
+        assert torch.equal(y, want) and torch.equal(want, _layer(seed)(x)), (seed, len(noise))

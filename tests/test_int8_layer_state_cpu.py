@@ -108,3 +108,16 @@ def test_nothing_made_inside_a_capture_is_kept(calls, monkeypatch):
     layer.prepack()
     assert layer.codes8 is None
     monkeypatch.undo()
+
+
+def test_codes_keep_their_memory(calls):
+    """New planes of the same shape are quantized into the tensors that graphs may read."""
+    layer = _layer()
+    _run(layer)
+    layer.bias.fill_(1)
+    _run(layer)
+    kept = layer.codes8, layer.scale8, layer._bias_f32()
+    layer.u_s0.codes.add_(1)
+    layer.bias.fill_(2)
+    assert _same(_run(layer), layer)
+    assert all(a is b for a, b in zip(kept, (layer.codes8, layer.scale8, layer._bias_f32()))) and (kept[2] == 2).all()

@@ -25,8 +25,9 @@ from .packing import AXIAL_STAGES, BLOCK_SIZE, SUPPORTED_QUANT_METHODS, PackedLa
 def _made_from(tensors):
     """A record of the tensors that something kept was made from, for :func:`_unchanged`. It holds
     them and an alias of their memory, so neither they nor their addresses can come back with
-    other values while the record lives."""
-    return [(t, t._version, t.data_ptr(), t.detach()) for t in tensors]
+    other values while the record lives. Tensors made in inference mode have no version: writes
+    into them do not show."""
+    return [(t, None if t.is_inference() else t._version, t.data_ptr(), t.detach()) for t in tensors]
 
 
 def _unchanged(record, tensors) -> bool:
@@ -34,7 +35,7 @@ def _unchanged(record, tensors) -> bool:
     if record is None:
         return False
     for t, (s, version, address, _) in zip(tensors, record):
-        if t is not s or t._version != version or t.data_ptr() != address:
+        if t is not s or (version is not None and t._version != version) or t.data_ptr() != address:
             return False
     return True
 
@@ -91,7 +92,10 @@ class PackedPhaseLinear(nn.Module):
     coefficients are quantized once to int8 with a scale per output channel
     (half the memory of the fp16 matrix), every call quantizes its activations
     to 8 bits with a scale per token (``ops.linear_int8``). It takes the place of
-    the activation quantizers above and needs ``cache_dense=True``.
+    the activation quantizers above and needs ``cache_dense=True``. Planes that
+    are loaded, written, moved or replaced are quantized again by the next call;
+    only a write into planes that were made in inference mode does not show:
+    call :meth:`prepack` after it.
     """
 
     def __init__(self, in_features: int, out_features: int, stages: int = 2, code_bits: int = 2,
@@ -175,7 +179,7 @@ class PackedPhaseLinear(nn.Module):
         if self._bias32 is not None and _unchanged(self._bias32[0], (self.bias,)):
             return self._bias32[1]
         bias = self.bias.float()
-        if not _capturing(self.bias):
+        if not _capturing(self.bias) and not self.bias.is_inference():
             record = _made_from((self.bias,))
             (bias,) = _keep(None if self._bias32 is None else self._bias32[1:], (bias,))
             self._bias32 = (record, bias)
@@ -207,6 +211,10 @@ class PackedPhaseLinear(nn.Module):
         if self._bias32 is not None and not _unchanged(self._bias32[0], (self.bias,)):
             self._bias32 = None
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._planes8 = None
+        super()._load_from_state_dict(*args, **kwargs)
 
     def __getstate__(self):  # a copy makes its own codes and fp32 bias
         return {**self.__dict__, "_planes8": None, "_bias32": None}

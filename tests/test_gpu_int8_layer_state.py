@@ -109,3 +109,20 @@ def test_graph_reads_the_codes_of_loaded_planes(cuda):
         noise = [torch.full_like(layer.codes8, 17), torch.full_like(layer.scale8, 3.0), torch.full_like(want[0], 5.0)]
         g.replay()
         assert torch.equal(y, want) and torch.equal(want, _layer(seed)(x)), (seed, len(noise))
+
+
+def test_layer_made_in_inference_mode(cuda):
+    x = _x()
+    with torch.inference_mode():
+        layer = _layer(1)
+        assert torch.equal(layer(x), _layer(1)(x))
+        layer.load_state_dict(_layer(2).state_dict())
+    assert torch.equal(layer(x), _layer(2)(x))
+    with torch.inference_mode():
+        layer.load_state_dict(_layer(3).state_dict())
+        assert torch.equal(layer(x), _layer(3)(x))
+        layer.u_s0.codes.fill_(0)
+        layer.prepack()
+        other = _layer(3)
+        other.u_s0.codes.fill_(0)
+        assert torch.equal(layer(x), other(x))

@@ -1,6 +1,9 @@
 """What an 8-bit layer keeps between calls, on the CPU: the decoder, the row quantizer and the
 product are stand-ins on CPU tensors (the layer's own bookkeeping is the tested code)."""
 
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -121,3 +124,35 @@ def test_codes_keep_their_memory(calls):
     layer.bias.fill_(2)
     assert _same(_run(layer), layer)
     assert all(a is b for a, b in zip(kept, (layer.codes8, layer.scale8, layer._bias_f32()))) and (kept[2] == 2).all()
+
+
+def test_layer_made_in_inference_mode(calls):
+    """Its planes keep no version: calls run, in and outside of the mode, and loads are followed."""
+    with torch.inference_mode():
+        layer = _layer(1)
+        assert _same(_run(layer), layer)
+    assert _same(_run(layer), layer) and len(calls) == 1
+    for seed in (2, 3):
+        with torch.inference_mode():
+            layer.load_state_dict(_layer(seed).state_dict())
+            layer.bias.fill_(seed)
+        got = _run(layer)
+        assert _same(got, layer) and (got[2] == seed).all()
+    outside = _layer(4)
+    with torch.inference_mode():
+        assert _same(_run(outside), outside)
+    outside.u_s0.codes.add_(1)
+    outside.bias.fill_(9)
+    got = _run(outside)
+    assert _same(got, outside) and (got[2] == 9).all()
+
+
+def test_copies_make_their_own_codes(calls):
+    layer = _layer(1)
+    _run(layer)
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        other.u_s0.codes.add_(1)
+        other.bias.fill_(3)
+        got = _run(other)
+        assert _same(got, other) and (got[2] == 3).all()
+        assert _same(_run(layer), layer) and layer._bias_f32().ne(3).any()

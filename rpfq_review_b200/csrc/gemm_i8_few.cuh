@@ -177,14 +177,11 @@ __global__ void __launch_bounds__(kFewThreads) gemm_i8_few_kernel(const GemmI8Fe
     float b = 0.0f;
     if (p.g.bias != nullptr)
         b = p.g.bias_f32 ? static_cast<const float*>(p.g.bias)[col] : __half2float(static_cast<const __half*>(p.g.bias)[col]);
-    float v[4] = {fmaf(__int2float_rn(mine) * p.g.w_scale[col], s_scale[r], b), 0.0f, 0.0f, 0.0f};
-    // one column: the others lie past n
-    float res[4] = {};
-    if (p.g.residual != nullptr) load_i8_residual<OUT_F32, false>(p.g, r, col, p.g.n, res);
-    if (p.g.residual != nullptr)
-        store_i8_outputs<OUT_F32, true, false>(p.g, r, col, p.g.n, v, res);
-    else
-        store_i8_outputs<OUT_F32, false, false>(p.g, r, col, p.g.n, v, res);
+    float v = fmaf(__int2float_rn(mine) * p.g.w_scale[col], s_scale[r], b), unused = 0.0f;
+    if (p.g.activation == kActGelu) gelu_log_pair(v, unused);
+    using Out = typename std::conditional<OUT_F32, float, __half>::type;
+    if (p.g.residual != nullptr) v += static_cast<float>(static_cast<const Out*>(p.g.residual)[r * p.g.ldr + col]);
+    static_cast<Out*>(p.g.y)[r * p.g.ldy + col] = static_cast<Out>(v);
 }
 
 }  // namespace rpfq

@@ -177,8 +177,9 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
 /* y[m, n] = act(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]) +
  * residual[m, n] of int8 codes x [m, k] and w [n, k] with one scale per token
  * and one per output channel: exact int32 sums on the tensor cores, scaled in
- * fp32, fp16 or fp32 output. The 8-bit form of rpfq_gemm_sm100; y may alias
- * residual, but not overlap x. Requirements: x and w 16-byte aligned with row strides that are
+ * fp32, fp16 or fp32 output. The 8-bit form of rpfq_gemm_sm100; y may be the
+ * residual (the same address and row stride), and shares no other memory with what the call
+ * reads or with scratch. Requirements: x and w 16-byte aligned with row strides that are
  * multiples of 16 (any k up to 131071 within such rows); y, residual, bias and
  * the scales aligned to their values, any n and any row strides >= n; the
  * residual has y's dtype. Nothing is kept between calls.

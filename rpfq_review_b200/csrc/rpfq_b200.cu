@@ -14,6 +14,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <type_traits>
@@ -1086,17 +1087,63 @@ I8Plan plan_i8(const RpfqGemmI8Args* a, DeviceState* st) {
     return best;
 }
 
-// Whether some row of one matrix shares bytes with some row of another: `rows` rows of
-// a_bytes / b_bytes at strides a_step / b_step bytes. Exact for equal strides (columns
-// of one buffer), by their whole ranges otherwise.
-bool rows_overlap(const void* a, int64_t a_step, int64_t a_bytes, const void* b, int64_t b_step, int64_t b_bytes,
-                  int64_t rows) {
-    const intptr_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
-    const int64_t a_all = (rows - 1) * a_step + a_bytes, b_all = (rows - 1) * b_step + b_bytes;
-    if (pa + a_all <= pb || pb + b_all <= pa) return false;
-    if (a_step != b_step || rows == 1) return true;
-    const int64_t shift = ((pb - pa) % a_step + a_step) % a_step;  // b's columns within a's rows
-    return shift < a_bytes || shift + b_bytes > a_step;
+// Two arrays of runs of bytes: an axis of both, with the runs of either and their steps
+// in bytes.
+struct RunAxis {
+    int64_t a_count, a_step, b_count, b_step;
+};
+
+// With the axes from `at` on, whether a run of b, whose first begins d bytes behind a's
+// first, meets a run of a. Every step is at least as long as what lies within it, so only
+// the two neighbours of d along an axis can.
+bool runs_meet(const RunAxis* axes, int at, int n, __int128 d, __int128 a_bytes, __int128 b_bytes) {
+    if (at == n) return d < a_bytes && -d < b_bytes;
+    const __int128 step = axes[at].a_step;
+    __int128 t = -d / step;
+    if (t * step > -d) --t;  // rounded down
+    for (int i = 0; i < 2; ++i, ++t)
+        if (t > -axes[at].a_count && t < axes[at].b_count && runs_meet(axes, at + 1, n, d + t * step, a_bytes, b_bytes))
+            return true;
+    return false;
+}
+
+// Whether a run of array a (runs of a_bytes) shares bytes with one of array b, over at
+// most three axes. Exact where the axes have the same steps in both and are nested
+// (columns of one buffer, heads of one row); axes of different steps count with all that
+// lies between their runs, and axes that are not nested make any meeting of the arrays'
+// ranges one of runs.
+bool share_bytes(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes, std::initializer_list<RunAxis> list) {
+    RunAxis axes[3];
+    int n = 0;
+    __int128 a_lo = reinterpret_cast<intptr_t>(a), a_hi = a_lo + a_bytes, a_run = a_bytes;
+    __int128 b_lo = reinterpret_cast<intptr_t>(b), b_hi = b_lo + b_bytes, b_run = b_bytes;
+    const __int128 d = b_lo - a_lo;
+    bool nested = true;
+    for (RunAxis x : list) {
+        if (x.a_count <= 0 || x.b_count <= 0) return false;
+        const __int128 a_all = static_cast<__int128>(x.a_count - 1) * x.a_step;
+        const __int128 b_all = static_cast<__int128>(x.b_count - 1) * x.b_step;
+        (a_all < 0 ? a_lo : a_hi) += a_all;
+        (b_all < 0 ? b_lo : b_hi) += b_all;
+        if (x.a_count == 1) x.a_step = x.b_step;
+        if (x.b_count == 1) x.b_step = x.a_step;
+        if (x.a_count == 1 && x.b_count == 1) continue;
+        if (x.a_step < 0 || x.b_step < 0)
+            nested = false;
+        else if (x.a_step != x.b_step)
+            a_run += a_all, b_run += b_all;
+        else
+            axes[n++] = x;
+    }
+    if (a_hi <= b_lo || b_hi <= a_lo) return false;
+    std::sort(axes, axes + n, [](const RunAxis& x, const RunAxis& y) { return x.a_step > y.a_step; });
+    __int128 a_in = a_run, b_in = b_run;
+    for (int i = n - 1; i >= 0; --i) {
+        nested = nested && axes[i].a_step >= std::max(a_in, b_in);
+        a_in += static_cast<__int128>(axes[i].a_count - 1) * axes[i].a_step;
+        b_in += static_cast<__int128>(axes[i].b_count - 1) * axes[i].b_step;
+    }
+    return !nested || runs_meet(axes, 0, n, d, a_run, b_run);
 }
 
 int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
@@ -1134,10 +1181,22 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
     if (a->residual && (((a->flags & RPFQ_GEMM_RESIDUAL_F32) != 0) != ((a->flags & RPFQ_GEMM_OUT_F32) != 0)))
         return fail(RPFQ_ERR_UNSUPPORTED, "%s: the residual must have the output's dtype", who);
-    // rows of x are read until the last output is written
-    if (rows_overlap(a->x, a->ldx * static_cast<int64_t>(xsize), a->k * static_cast<int64_t>(xsize), a->y,
-                     a->ldy * static_cast<int64_t>(esize), a->n * static_cast<int64_t>(esize), a->m))
+    // the operands are read until the last output is written
+    const int64_t y_step = a->ldy * static_cast<int64_t>(esize), y_row = a->n * static_cast<int64_t>(esize);
+    auto in_y = [&](const void* from, int64_t rows, int64_t step, int64_t bytes) {
+        return from && share_bytes(from, bytes, a->y, y_row, {{rows, step, a->m, y_step}});
+    };
+    if (in_y(a->x, a->m, a->ldx * static_cast<int64_t>(xsize), a->k * static_cast<int64_t>(xsize)))
         return fail(RPFQ_ERR_INVALID, "%s: y must not overlap x", who);
+    const char* shared = in_y(a->w, a->n, a->ldw, a->k)                                    ? "w"
+                         : in_y(a->w_scale, 1, 0, a->n * int64_t(4))                       ? "w_scale"
+                         : !x_flags && in_y(a->x_scale, 1, 0, a->m * 4)                    ? "x_scale"
+                         : in_y(a->bias, 1, 0, a->n * static_cast<int64_t>(bsize))         ? "bias"
+                                                                                           : nullptr;
+    if (shared) return fail(RPFQ_ERR_INVALID, "%s: y shares memory with %s", who, shared);
+    if (!(a->residual == a->y && (a->ldr == a->ldy || a->m == 1)) &&
+        in_y(a->residual, a->m, a->ldr * static_cast<int64_t>(esize), y_row))
+        return fail(RPFQ_ERR_INVALID, "%s: y shares memory with other rows or columns of the residual", who);
     if (a->block_n != 0 && a->block_n != 64 && a->block_n != 128 && a->block_n != 256)
         return fail(RPFQ_ERR_INVALID, "%s: block_n must be 0, 64, 128 or 256 (got %d)", who, a->block_n);
     if (a->split_k < 0 || a->split_k > kMaxSplits || (a->split_k > 1 && a->block_n == 256))
@@ -1148,6 +1207,10 @@ int gemm_i8(const RpfqGemmI8Args* args, cudaStream_t stream) {
     if (need && (!a->scratch || !aligned16(a->scratch) || a->scratch_bytes < need))
         return fail(RPFQ_ERR_INVALID, "%s: quantizing %lld rows needs 16-byte aligned scratch of %llu bytes", who,
                     (long long)a->m, (unsigned long long)need);
+    if (need && (in_y(a->scratch, 1, 0, static_cast<int64_t>(need)) ||
+                 share_bytes(a->scratch, static_cast<int64_t>(need), a->x, a->k * static_cast<int64_t>(xsize),
+                             {{1, 0, a->m, a->ldx * static_cast<int64_t>(xsize)}})))
+        return fail(RPFQ_ERR_INVALID, "%s: scratch shares memory with x or y", who);
     DeviceState* st;
     int rc = device_state(&st);
     if (rc) return rc;

@@ -679,9 +679,9 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     channel (``rpfq_gemm_i8_sm100``): exact int32 sums on the tensor cores
     (k up to ``GEMM_INT8_MAX_K``), scaled in fp32. ``bias`` fp16 or fp32;
     ``residual`` and ``out`` fp16 or fp32 alike (and may be the same tensor for
-    an in-place residual add; ``out`` must not overlap ``x``). Code rows that do
-    not start on 16 bytes are copied into rows that do; :func:`quantize_rows`
-    returns such rows.
+    an in-place residual add; ``out`` must not share memory with anything else that
+    the call reads). Code rows that do not start on 16 bytes are copied into rows
+    that do; :func:`quantize_rows` returns such rows.
     ``block_n`` (64, 128, 256) and ``split_k`` (1..8) fix the tiles and the parts
     of k, 0 leaves them to the library; the result is the same bit for bit."""
     name = "gemm_int8"

@@ -1,0 +1,46 @@
+"""GPU tests: outputs beside what a call reads, in one buffer, are answered; outputs over it are
+refused."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("m", [1, 4, 40, 1200])
+def test_int8_output_beside_its_operands(cuda, m):
+    from rpfq_review_b200 import ops
+    n, k = 48, 64
+    w, ws = ops.quantize_rows(torch.randn(n, k, device=cuda))
+    x, xs = ops.quantize_rows(torch.randn(m, k, device=cuda))
+    res = torch.randn(m, n, device=cuda).half()
+    want = ops.gemm_int8(x, xs, w, ws, residual=res)
+    buf = torch.zeros(m, 3 * n, dtype=torch.float16, device=cuda)
+    for out_at, res_at in ((0, n), (2 * n, 0), (n, 2 * n), (n, 0), (n, n)):
+        r, out = buf[:, res_at:res_at + n], buf[:, out_at:out_at + n]
+        r.copy_(res)
+        assert torch.equal(ops.gemm_int8(x, xs, w, ws, residual=r, out=out), want)
+        assert out_at == res_at or torch.equal(r, res)
+    # rows of w and of the output in one matrix, of the same stride
+    both = torch.zeros(max(m, n), 64 + 96, dtype=torch.int8, device=cuda)
+    both[:n, :k] = w
+    out = both[:m, 64:].view(torch.float16)
+    assert torch.equal(ops.gemm_int8(x, xs, both[:n, :k], ws, residual=res, out=out), want)
+    assert torch.equal(both[:n, :k], w)
+
+
+def test_int8_output_over_its_operands_is_refused(cuda):
+    from rpfq_review_b200 import ops
+    m, n, k = 40, 48, 64
+    w, ws = ops.quantize_rows(torch.randn(n, k, device=cuda))
+    x, xs = ops.quantize_rows(torch.randn(m, k, device=cuda))
+    buf = torch.zeros(m + 1, 2 * n, dtype=torch.float16, device=cuda)
+    flat = torch.zeros(m * n + 1, device=cuda).half()
+    bias = torch.zeros(m * n, device=cuda)
+    for residual, out, more in ((buf[:m, :n], buf[:m, 8:n + 8], {}), (buf[:m, :n], buf[1:, :n], {}),
+                                (flat[1:].view(m, n), flat[:-1].view(m, n), {}),
+                                (None, bias.view(m, n), dict(bias=bias[:n]))):
+        with pytest.raises(ValueError, match="shares memory"):
+            ops.gemm_int8(x, xs, w, ws, residual=residual, out=out, **more)
+    with pytest.raises(ValueError, match="with w"):
+        ops.gemm_int8(x[:10], xs[:10], w, ws, out=w.view(-1)[:10 * n * 2].view(torch.float16).view(10, n))

@@ -1,0 +1,45 @@
+"""CPU tests: the C entry points of the 8-bit path and the rotary positions refuse outputs over
+what they read. Addresses are invented; every call here is refused before any device work."""
+
+import ctypes
+
+import pytest
+
+from rpfq_review_b200 import _lib
+
+MB = 1 << 20
+
+
+def _gemm(**kw):
+    """x [4, 60] in rows of 64, w [32, 60] in rows of 64, y and residual fp16 [4, 32] in rows of
+    32, all apart."""
+    a = dict(x=MB, ldx=64, x_scale=2 * MB, w=3 * MB, ldw=64, w_scale=4 * MB, bias=5 * MB, residual=6 * MB, ldr=32,
+             y=7 * MB, ldy=32, m=4, n=32, k=60, activation=0, flags=0)
+    a.update(kw)
+    rc = _lib.lib().rpfq_gemm_i8_sm100(ctypes.byref(_lib.RpfqGemmI8Args(**a)), None)
+    return rc, _lib.lib().rpfq_last_error()
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(y=MB), b"overlap x"), (dict(y=MB - 4 * 64 + 64), b"overlap x"), (dict(y=MB + 4 * 64 - 8), b"overlap x"),
+    (dict(y=3 * MB), b"with w"), (dict(y=3 * MB + 31 * 64 + 58), b"with w"), (dict(y=3 * MB - 3 * 64 - 62), b"with w"),
+    (dict(y=4 * MB + 126), b"w_scale"), (dict(y=4 * MB - 254), b"w_scale"), (dict(y=2 * MB + 14), b"x_scale"),
+    (dict(y=5 * MB + 62), b"bias"), (dict(y=5 * MB + 126, flags=4), b"bias"),
+    (dict(y=6 * MB + 2), b"residual"), (dict(y=6 * MB - 64), b"residual"), (dict(y=6 * MB, ldy=40), b"residual"),
+    (dict(y=6 * MB + 64), b"residual"), (dict(y=6 * MB, ldr=64, ldy=32), b"residual"),
+    (dict(residual=7 * MB + 62, ldr=64, ldy=64), b"residual"), (dict(residual=7 * MB + 66, ldr=64, ldy=64), b"residual"),
+    (dict(flags=8, m=9, x_scale=None, scratch=7 * MB, scratch_bytes=MB), b"scratch"),
+    (dict(flags=8, m=9, x_scale=None, scratch=MB - 16, scratch_bytes=MB), b"scratch"),
+    # w in y's rows of another stride, and the other way round
+    (dict(x=MB, y=3 * MB + 60, ldy=64), b"with w"), (dict(w=7 * MB + 64, ldw=128), b"with w")])
+def test_gemm_i8_refuses_an_output_over_an_operand(bad, word):
+    rc, message = _gemm(**bad)
+    assert rc == _lib.RPFQ_ERR_INVALID and word in message, message
+
+
+def test_gemm_i8_invented_addresses_are_refused():
+    """Columns beside x whose rows reach into w (x, w and the scales at one address)."""
+    for y, n in ((4096 + 64, 32), (4096 + 60, 34)):
+        rc, message = _gemm(x=4096, x_scale=4096, w=4096, w_scale=4096, bias=None, residual=None, ldr=0, y=y, n=n,
+                            ldx=128, ldy=64)
+        assert rc == _lib.RPFQ_ERR_INVALID and b"with w" in message

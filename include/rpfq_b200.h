@@ -231,7 +231,8 @@ enum { RPFQ_POS_I32 = 0, RPFQ_POS_I64 = 1, RPFQ_POS_F32 = 2, RPFQ_POS_F64 = 3 };
  * positions[.., 1]. Angles are formed and reduced in fp64. x and y are fp16
  * (fp32 with f32 != 0) [batch, length, heads, dim] with strides in elements
  * and unit stride inside a head; y may be x (same strides), which leaves the
- * values past 2 * pairs untouched, and may not overlap x in any other way. */
+ * values past 2 * pairs untouched, and shares memory with nothing that is read in any
+ * other way. */
 typedef struct RpfqRotaryArgs {
     const void* x;
     int64_t x_batch, x_token, x_head;   /* strides                                        */

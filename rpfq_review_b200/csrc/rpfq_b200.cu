@@ -1526,6 +1526,20 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     if (a->x == a->y && ((a->batch > 1 && a->x_batch != a->y_batch) || (a->length > 1 && a->x_token != a->y_token) ||
                          (a->heads > 1 && a->x_head != a->y_head)))
         return fail(RPFQ_ERR_INVALID, "%s: in place, x and y must have the same strides", who);
+    const int64_t run = a->dim * static_cast<int64_t>(esize);
+    if (a->x != a->y && share_bytes(a->x, run, a->y, run,
+                                    {{a->batch, a->x_batch * esize, a->batch, a->y_batch * esize},
+                                     {a->length, a->x_token * esize, a->length, a->y_token * esize},
+                                     {a->heads, a->x_head * esize, a->heads, a->y_head * esize}}))
+        return fail(RPFQ_ERR_INVALID, "%s: y must be x or not overlap x", who);
+    auto in_y = [&](const void* from, int64_t bytes) {
+        return share_bytes(from, bytes, a->y, run,
+                           {{1, 0, a->batch, a->y_batch * esize}, {1, 0, a->length, a->y_token * esize},
+                            {1, 0, a->heads, a->y_head * esize}});
+    };
+    if (in_y(a->positions, ((a->batch - 1) * a->position_batch + a->length * a->axes) * psize))
+        return fail(RPFQ_ERR_INVALID, "%s: y shares memory with positions", who);
+    if (in_y(a->inv_freq, a->pairs * int64_t(8))) return fail(RPFQ_ERR_INVALID, "%s: y shares memory with inv_freq", who);
     DeviceState* st;
     int rc = device_state(&st);
     if (rc) return rc;

@@ -780,7 +780,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     of the pairs takes the first (a patch's row) and the rest the second (its
     column). ``out`` may be ``x`` (in place), e.g. the query and key heads of a
     qkv product's rows: ``q = qkv.view(B, L, 3 * H, D)[:, :, :2 * H]``. It must
-    not overlap x in any other way.
+    not overlap x in any other way, nor the positions or frequencies.
 
     No autograd: ``transpose=True`` turns the other way, which maps the gradient
     of the output to the gradient of x."""

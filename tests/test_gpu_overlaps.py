@@ -44,3 +44,34 @@ def test_int8_output_over_its_operands_is_refused(cuda):
             ops.gemm_int8(x, xs, w, ws, residual=residual, out=out, **more)
     with pytest.raises(ValueError, match="with w"):
         ops.gemm_int8(x[:10], xs[:10], w, ws, out=w.view(-1)[:10 * n * 2].view(torch.float16).view(10, n))
+
+
+@pytest.mark.parametrize("D", [64, 20, 7])
+def test_rotary_output_beside_its_input(cuda, D):
+    """Query heads into the place of the key heads of the same rows, heads and tokens of one
+    buffer in turn, an expanded input: answered. Shifted by a head, a token or a value: refused."""
+    from rpfq_review_b200 import ops
+    B, L, H, P = 2, 9, 3, D // 2
+    f = ops.rotary_frequencies(2 * P, device=cuda)[0]
+    pos = torch.arange(L, device=cuda)
+    x = torch.randn(B, L, H, D, device=cuda).half()
+    want = ops.rotary(x, pos, f)
+    rows = torch.zeros(B, L, 3 * H, D, dtype=torch.float16, device=cuda)
+    tokens = torch.zeros(B, 2 * L, H, D, dtype=torch.float16, device=cuda)
+    for src, out in ((rows[:, :, :H], rows[:, :, H:2 * H]), (rows[:, :, 2 * H:], rows[:, :, :H]),
+                     (rows[:, :, 0:2 * H:2], rows[:, :, 1:2 * H:2]), (tokens[:, ::2], tokens[:, 1::2]),
+                     (tokens[:, L:], tokens[:, :L]), (rows[:, :, :H], rows[:, :, :H])):
+        src.copy_(x)
+        assert torch.equal(ops.rotary(src, pos, f, out=out), want)
+        assert out.data_ptr() == src.data_ptr() or torch.equal(src, x)
+    one = x[:1].expand(B, L, H, D)
+    assert torch.equal(ops.rotary(one, pos, f, out=rows[:, :, :H]), ops.rotary(x[:1], pos, f).expand(B, L, H, D))
+    flat = torch.zeros(B * L * H * D + 8, dtype=torch.float16, device=cuda)
+    for src, out in ((rows[:, :, :H], rows[:, :, 1:H + 1]), (tokens[:, :L], tokens[:, 1:L + 1]),
+                     (flat[:-8].view(B, L, H, D), flat[1:-7].view(B, L, H, D)),
+                     (flat[8:].view(B, L, H, D), flat[:-8].view(B, L, H, D))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.rotary(src, pos, f, out=out)
+    shared = torch.zeros(64, dtype=torch.float64, device=cuda)
+    with pytest.raises(ValueError, match="inv_freq"):
+        ops.rotary(x[0, :1, :1], pos[:1], shared[:P], out=shared.view(torch.float16)[:D].view(1, 1, D))

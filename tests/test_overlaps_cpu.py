@@ -43,3 +43,27 @@ def test_gemm_i8_invented_addresses_are_refused():
         rc, message = _gemm(x=4096, x_scale=4096, w=4096, w_scale=4096, bias=None, residual=None, ldr=0, y=y, n=n,
                             ldx=128, ldy=64)
         assert rc == _lib.RPFQ_ERR_INVALID and b"with w" in message
+
+
+def _rotary(**kw):
+    """x and y [2, 5, 2, 64] fp16 in rows of 128, apart; positions int32 [5], 32 frequencies."""
+    a = dict(x=MB, x_batch=640, x_token=128, x_head=64, y=2 * MB, y_batch=640, y_token=128, y_head=64, positions=3 * MB,
+             position_batch=0, inv_freq=4 * MB, batch=2, length=5, heads=2, dim=64, pairs=32, axes=1, position_type=0,
+             f32=0, interleaved=0, transpose=0, magnitude=1.0)
+    a.update(kw)
+    rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(_lib.RpfqRotaryArgs(**a)), None)
+    return rc, _lib.lib().rpfq_last_error()
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(y=MB + 2), b"overlap x"), (dict(y=MB + 128), b"overlap x"), (dict(y=MB - 128), b"overlap x"),
+    (dict(y=MB + 256), b"overlap x"), (dict(y=MB + 1280), b"overlap x"), (dict(y=MB + 2 * 1280 - 2), b"overlap x"),
+    (dict(y=MB - 2 * 1280 + 2), b"overlap x"), (dict(y=MB + 2, x_token=256, x_batch=1280), b"overlap x"),
+    (dict(x_token=192, y_token=192, x_batch=960, y_batch=960, y=MB + 128), b"overlap x"),
+    (dict(x=MB, y=MB + 130, x_token=128, y_token=128, heads=1), b"overlap x"),
+    (dict(y=3 * MB - 2 * 1280 + 2), b"positions"), (dict(y=3 * MB + 18), b"positions"),
+    (dict(y=3 * MB + 38, position_batch=5), b"positions"), (dict(y=4 * MB + 254), b"inv_freq"),
+    (dict(y=4 * MB - 2 * 1280 + 2), b"inv_freq")])
+def test_rotary_refuses_an_output_over_what_it_reads(bad, word):
+    rc, message = _rotary(**bad)
+    assert rc == _lib.RPFQ_ERR_INVALID and word in message, message

@@ -836,7 +836,7 @@ int quantize_rows(const char* who, const void* x, bool f32, int64_t ldx, int8_t*
     const bool twice = vecs > 32 * kQuantKeep;
     if (vecs > 64 * kQuantKeep || mode == kQuantSingle || m * threads < int64_t(256) * st->sm_count) threads = 256;
     const int64_t blocks = (m * threads + 255) / 256;
-    if (blocks > 0x7fffffff || k > (1 << 30)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or k too large", who);
+    if (blocks > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m too large", who);
     RPFQ_CUDA((f32 ? launch_quantize_rows<float>(mode, threads, twice, blocks, stream, p)
                    : launch_quantize_rows<__half>(mode, threads, twice, blocks, stream, p)));
     return RPFQ_OK;
@@ -1486,6 +1486,8 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
     if (m == 0) return RPFQ_OK;
     if (!x || !q || !scale) return fail(RPFQ_ERR_INVALID, "%s: null pointer", who);
     if (ldx < k || ldq < k) return fail(RPFQ_ERR_INVALID, "%s: row strides must be >= k", who);
+    // 32 rows of a block at most, 2^31 blocks
+    if (m > int64_t(1) << 36 || k > (1 << 30)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or k too large", who);
     if (reinterpret_cast<uintptr_t>(x) % (x_f32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4)
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
     DeviceState* st;
@@ -1496,7 +1498,7 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
 
 uint64_t rpfq_gemm_i8_scratch_bytes(int64_t m, int32_t k) {
     if (m <= 0 || k <= 0 || few_rows_fit(m, k, true)) return 0;
-    return static_cast<uint64_t>(m) * ((k + 15) / 16 * 16 + 4);
+    return static_cast<uint64_t>(m) * ((static_cast<int64_t>(k) + 15) / 16 * 16 + 4);
 }
 
 int rpfq_gemm_i8_sm100(const RpfqGemmI8Args* args, rpfq_stream_t stream) {
@@ -1517,6 +1519,8 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     if (a->position_type < RPFQ_POS_I32 || a->position_type > RPFQ_POS_F64)
         return fail(RPFQ_ERR_INVALID, "%s: unknown position type %d", who, a->position_type);
     if (a->batch == 0 || a->length == 0 || a->heads == 0) return RPFQ_OK;
+    if (a->length > 0x7fffffff || a->batch > 0x7fffffff / a->length)
+        return fail(RPFQ_ERR_UNSUPPORTED, "%s: too many tokens", who);
     if (!a->x || !a->y || !a->positions || !a->inv_freq) return fail(RPFQ_ERR_INVALID, "%s: null pointer", who);
     const int esize = a->f32 ? 4 : 2;
     const int psize = (a->position_type == RPFQ_POS_I32 || a->position_type == RPFQ_POS_F32) ? 4 : 8;
@@ -1562,7 +1566,6 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     p.copy_rest = copy_rest ? 1 : 0;
     p.magnitude = a->magnitude;
     p.sign = a->transpose ? -1.0f : 1.0f;
-    if (p.tokens > 0x7fffffff || a->length > 0x7fffffff) return fail(RPFQ_ERR_UNSUPPORTED, "%s: too many tokens", who);
     const int bytes = rotary_vec(a, esize, 16, copy_rest) ? 16 : (rotary_vec(a, esize, 8, copy_rest) ? 8 : 0);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     RPFQ_CUDA((a->f32 ? (a->interleaved ? launch_rotary<float, true>(bytes, st, cs, p)

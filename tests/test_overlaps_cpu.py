@@ -67,3 +67,18 @@ def _rotary(**kw):
 def test_rotary_refuses_an_output_over_what_it_reads(bad, word):
     rc, message = _rotary(**bad)
     assert rc == _lib.RPFQ_ERR_INVALID and word in message, message
+
+
+@pytest.mark.parametrize("batch,length", [(2 ** 62 + 1, 4), (2 ** 62, 4), (2 ** 32, 2 ** 32 + 1), (2 ** 31, 1), (1, 2 ** 31),
+                                          (2 ** 16, 2 ** 15)])
+def test_rotary_refuses_more_tokens_than_it_counts(batch, length):
+    """Products past 2^64 among them, which would come out small."""
+    rc, message = _rotary(batch=batch, length=length, x_batch=0, y_batch=128)
+    assert rc == _lib.RPFQ_ERR_UNSUPPORTED and b"tokens" in message, message
+
+
+@pytest.mark.parametrize("m,k", [(2 ** 61 + 1, 8), (2 ** 59 + 1, 8), (2 ** 56 + 1, 8), (2 ** 40, 8), (2, 2 ** 31 - 1)])
+def test_quantize_rows_refuses_more_rows_than_it_counts(m, k):
+    rc = _lib.lib().rpfq_quantize_rows_sm100(MB, 0, 2 ** 31 - 1, 2 * MB, 2 ** 31 - 1, 3 * MB, m, k, None)
+    assert rc == _lib.RPFQ_ERR_UNSUPPORTED and b"too large" in _lib.lib().rpfq_last_error()
+    assert _lib.lib().rpfq_gemm_i8_scratch_bytes(9, 2 ** 31 - 1) == 9 * (2 ** 31 + 4)

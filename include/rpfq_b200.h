@@ -168,7 +168,7 @@ int rpfq_act_quant_sm100(const uint16_t* x, int64_t ldx, uint16_t* xq, int64_t l
  * (fp32 with x_f32 != 0), row stride ldx; q is [m, k] int8, row stride ldq.
  *   t = max(amax |x|, 1e-30); q = rint(fl(x * fl(fl(1 / t) * 127))); scale = t / 127
  * (half to even, fp32 steps). A row with a NaN or an infinity gets codes of
- * zero and a scale of NaN. No counterpart in the reference, whose quantizers
+ * zero and a scale of NaN. q, scale and x share no memory. No counterpart in the reference, whose quantizers
  * return to fp16 (ActivationQuantSTE.forward,
  * RPFQ-ViT-main/quant_models/quant_i.py:442-455). */
 int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* q, int64_t ldq, float* scale,

@@ -1490,6 +1490,12 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
     if (m > int64_t(1) << 36 || k > (1 << 30)) return fail(RPFQ_ERR_UNSUPPORTED, "%s: m or k too large", who);
     if (reinterpret_cast<uintptr_t>(x) % (x_f32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4)
         return fail(RPFQ_ERR_INVALID, "%s: a pointer is not aligned to its values", who);
+    const int64_t row = k * int64_t(x_f32 ? 4 : 2), step = ldx * (x_f32 ? 4 : 2);
+    if (share_bytes(x, row, q, k, {{m, step, m, ldq}})) return fail(RPFQ_ERR_INVALID, "%s: q shares memory with x", who);
+    if (share_bytes(x, row, scale, m * 4, {{m, step, 1, 0}}))
+        return fail(RPFQ_ERR_INVALID, "%s: scale shares memory with x", who);
+    if (share_bytes(q, k, scale, m * 4, {{m, ldq, 1, 0}}))
+        return fail(RPFQ_ERR_INVALID, "%s: q and scale share memory", who);
     DeviceState* st;
     int rc = device_state(&st);
     if (rc) return rc;

@@ -75,3 +75,20 @@ def test_rotary_output_beside_its_input(cuda, D):
     shared = torch.zeros(64, dtype=torch.float64, device=cuda)
     with pytest.raises(ValueError, match="inv_freq"):
         ops.rotary(x[0, :1, :1], pos[:1], shared[:P], out=shared.view(torch.float16)[:D].view(1, 1, D))
+
+
+def test_codes_beside_their_rows(cuda):
+    """The codes and scales of rows into the same buffer, beside them: through the C entry."""
+    from rpfq_review_b200 import _lib, ops
+    m, k = 5000, 64
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(0)).half().to(cuda)
+    buf = torch.zeros(m, 2 * k + k + 16, dtype=torch.uint8, device=cuda)
+    rows, codes = buf[:, :2 * k].view(torch.float16), buf[:, 2 * k:3 * k].view(torch.int8)
+    rows.copy_(x)
+    scale = torch.empty(m, device=cuda)
+    _lib.check(_lib.lib().rpfq_quantize_rows_sm100(rows.data_ptr(), 0, buf.stride(0) // 2, codes.data_ptr(), buf.stride(0),
+                                                   scale.data_ptr(), m, k, torch.cuda.current_stream().cuda_stream),
+               "rpfq_quantize_rows_sm100")
+    want = ops.quantize_rows(x)
+    assert torch.equal(codes, want[0]) and torch.equal(scale, want[1]) and torch.equal(rows, x)
+    assert (buf[:, 3 * k:] == 0).all()

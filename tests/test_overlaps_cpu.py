@@ -82,3 +82,18 @@ def test_quantize_rows_refuses_more_rows_than_it_counts(m, k):
     rc = _lib.lib().rpfq_quantize_rows_sm100(MB, 0, 2 ** 31 - 1, 2 * MB, 2 ** 31 - 1, 3 * MB, m, k, None)
     assert rc == _lib.RPFQ_ERR_UNSUPPORTED and b"too large" in _lib.lib().rpfq_last_error()
     assert _lib.lib().rpfq_gemm_i8_scratch_bytes(9, 2 ** 31 - 1) == 9 * (2 ** 31 + 4)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("bad,word", [
+    (dict(q=MB), b"q shares"), (dict(q=MB + 8), b"q shares"), (dict(q=MB - 3 * 32 - 7), b"q shares"),
+    (dict(scale=MB + 4), b"scale shares"), (dict(scale=MB - 12), b"scale shares"),
+    (dict(scale=2 * MB + 4), b"q and scale"), (dict(q=3 * MB + 15), b"q and scale")])
+def test_quantize_rows_refuses_outputs_over_what_is_read(f32, bad, word):
+    """x [4, 8] in rows of 32 bytes, q in rows of 32, scale [4]."""
+    a = dict(x=MB, q=2 * MB, scale=3 * MB)
+    a.update(bad)
+    L = _lib.lib()
+    assert L.rpfq_quantize_rows_sm100(a["x"], f32, 8 if f32 else 16, a["q"], 32, a["scale"], 4, 8,
+                                      None) == _lib.RPFQ_ERR_INVALID
+    assert word in L.rpfq_last_error()

@@ -511,19 +511,16 @@ def act_quant(x: torch.Tensor, num_bits: int, out: torch.Tensor | None = None) -
 GEMM_INT8_MAX_K = 131071  # 128 * 128 * k < 2^31: the int32 sums cannot overflow
 
 
-def _tensors(name: str, index: int, differentiable, others) -> None:
+def _tensors(name: str, index: int, tensors) -> None:
     """Every tensor (None: not given) is on cuda:index, and no gradient is asked for
-    through the first ones: these operators have no autograd."""
+    through any: these operators have no autograd."""
     grad = torch.is_grad_enabled()
-    for t in differentiable:
+    for t in tensors:
         if t is not None:
             if t.get_device() != index:
                 raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
             if grad and t.requires_grad:
                 raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
-    for t in others:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
 
 
 def _float_type(t: torch.Tensor, name: str) -> bool:
@@ -581,7 +578,7 @@ def quantize_rows(x: torch.Tensor):
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return quantize_rows(x)
-    _tensors("quantize_rows", index, (x,), ())
+    _tensors("quantize_rows", index, (x,))
     shape = x.shape
     if not shape or shape[-1] == 0:
         raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(shape)}")
@@ -607,7 +604,7 @@ def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int,
         with torch.cuda.device(index):
             return _gemm_int8(name, index, x, x2, m, ldx, x_scale, x_flag, w, w_scale, bias, residual, activation, out,
                               out_dtype, block_n, split_k)
-    _tensors(name, index, (x, w_scale, residual), (w, bias, out))
+    _tensors(name, index, (x, w, w_scale, bias, residual, out))
     n, k = w.shape
     if w_scale.dtype is not torch.float32 or w_scale.numel() != n:
         raise ValueError(f"{name}: w_scale must hold {n} float32 values, got {w_scale.numel()} of {w_scale.dtype}")
@@ -683,12 +680,14 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     the call reads). Code rows that do not start on 16 bytes are copied into rows
     that do; :func:`quantize_rows` returns such rows.
     ``block_n`` (64, 128, 256) and ``split_k`` (1..8) fix the tiles and the parts
-    of k, 0 leaves them to the library; the result is the same bit for bit."""
+    of k, 0 leaves them to the library; the result is the same bit for bit.
+
+    No autograd: a tensor that asks for a gradient is refused."""
     name = "gemm_int8"
     _require(x, "x", torch.int8)
     _check_codes(name, w)
     index = x.get_device()
-    _tensors(name, index, (x_scale,), ())
+    _tensors(name, index, (x_scale,))
     x2, m, ldx = _code_rows(x, w.shape[1], "x")
     if x_scale.dtype is not torch.float32 or x_scale.numel() != m:
         raise ValueError(f"{name}: x_scale must hold one float32 value per row ({m}), got {x_scale.numel()} of "
@@ -787,7 +786,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     name = "rotary"
     f32 = _float_type(x, "x")
     index = x.get_device()
-    _tensors(name, index, (x,), (positions, inv_freq, out))
+    _tensors(name, index, (x, positions, inv_freq, out))
     four = x.dim() == 4
     if not four and x.dim() != 3:
         raise ValueError(f"{name}: x must be [L, H, D] or [B, L, H, D], got {tuple(x.shape)}")

@@ -18,6 +18,7 @@ import os
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .packing import PackedLayer
@@ -513,14 +514,16 @@ GEMM_INT8_MAX_K = 131071  # 128 * 128 * k < 2^31: the int32 sums cannot overflow
 
 def _tensors(name: str, index: int, tensors) -> None:
     """Every tensor (None: not given) is on cuda:index, and no gradient is asked for
-    through any: these operators have no autograd."""
-    grad = torch.is_grad_enabled()
+    through any, nor a tangent given: these operators have no autograd."""
+    grad, forward = torch.is_grad_enabled(), forward_ad._current_level >= 0
     for t in tensors:
         if t is not None:
             if t.get_device() != index:
                 raise ValueError(f"{name}: every tensor must be on cuda:{index}, got one on {t.device}")
             if grad and t.requires_grad:
                 raise ValueError(f"{name} has no autograd: call it under torch.no_grad() or on detached tensors")
+            if forward and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no autograd: it takes no tensor with a tangent")
 
 
 def _float_type(t: torch.Tensor, name: str) -> bool:
@@ -682,7 +685,7 @@ def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     ``block_n`` (64, 128, 256) and ``split_k`` (1..8) fix the tiles and the parts
     of k, 0 leaves them to the library; the result is the same bit for bit.
 
-    No autograd: a tensor that asks for a gradient is refused."""
+    No autograd: a tensor that asks for a gradient or carries a tangent is refused."""
     name = "gemm_int8"
     _require(x, "x", torch.int8)
     _check_codes(name, w)

@@ -43,3 +43,16 @@ def test_gradients_are_refused(cuda):
                 pytest.fail(f"{name} took {which} with a gradient")
             with torch.no_grad():
                 call(**given)
+
+
+def test_tangents_are_refused(cuda):
+    """Forward mode: a dual tensor's tangent would be dropped."""
+    import torch.autograd.forward_ad as fwd
+    for name, (call, tensors) in _calls(cuda).items():
+        with fwd.dual_level(), torch.no_grad():
+            call(**tensors)
+            for which, t in tensors.items():
+                given = dict(tensors, **{which: fwd.make_dual(t.clone(), torch.ones_like(t))})
+                with pytest.raises(ValueError, match="no autograd"):
+                    call(**given)
+                    pytest.fail(f"{name} took {which} with a tangent")

@@ -19,6 +19,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .packing import PackedLayer
@@ -617,7 +618,8 @@ def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int,
     flags, bias_ptr, r_ptr, ldr = x_flag, None, None, 0
     w2, _, ldw = _code_rows(w, k, "w")
     w_scale = w_scale.contiguous()
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
         ldy = n
     else:
@@ -660,6 +662,8 @@ def _gemm_int8(name: str, index: int, x: torch.Tensor, x2: torch.Tensor, m: int,
     rc = L.rpfq_gemm_i8_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "rpfq_gemm_i8_sm100")
+    if given:
+        increment_version(out)
     if _timer is not None and m:
         _count_launch(2 if need else 1)
     return out
@@ -818,7 +822,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
         if out is x:
             raise ValueError(f"{name}: in place, a head must have unit stride")
         x = x.contiguous()
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError(f"{name}: out must be {tuple(x.shape)} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
@@ -836,6 +841,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
             rc = _lib.lib().rpfq_rotary_sm100(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "rpfq_rotary_sm100")
+    if given:
+        increment_version(out)
     if _timer is not None and x.numel():
         _count_launch()
     return out

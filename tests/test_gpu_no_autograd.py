@@ -56,3 +56,31 @@ def test_tangents_are_refused(cuda):
                 with pytest.raises(ValueError, match="no autograd"):
                     call(**given)
                     pytest.fail(f"{name} took {which} with a tangent")
+
+
+def test_written_outputs_are_seen_by_autograd(cuda):
+    """A backward pass that needs the old values of a tensor given as ``out`` says so."""
+    from rpfq_review_b200 import ops
+    calls = _calls(cuda)
+    for name in ("gemm_int8", "linear_int8", "rotary"):
+        call, tensors = calls[name]
+        out = tensors["out"].zero_()
+        a = torch.ones_like(out).requires_grad_()
+        loss = (a * out).sum()
+        with torch.no_grad():
+            version = out._version
+            assert call(**tensors) is out and out._version > version
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    heads, f = torch.randn(7, 2, 16, device=cuda), ops.rotary_frequencies(16, device=cuda)[0]
+    version = heads._version
+    ops.rotary(heads, torch.arange(7, device=cuda), f, out=heads)
+    assert heads._version > version
+    rows = torch.randn(7, 64, device=cuda)
+    version = rows._version
+    part = rows.view(7, 4, 16)[:, :2]
+    ops.rotary(part, torch.arange(7, device=cuda), f, out=part)
+    assert rows._version > version
+    with torch.inference_mode():
+        fresh = torch.randn(7, 2, 16, device=cuda)
+        ops.rotary(fresh, torch.arange(7, device=cuda), f, out=fresh)

@@ -1536,6 +1536,9 @@ int rpfq_rotary_sm100(const RpfqRotaryArgs* a, rpfq_stream_t stream) {
     if (a->x == a->y && ((a->batch > 1 && a->x_batch != a->y_batch) || (a->length > 1 && a->x_token != a->y_token) ||
                          (a->heads > 1 && a->x_head != a->y_head)))
         return fail(RPFQ_ERR_INVALID, "%s: in place, x and y must have the same strides", who);
+    if ((a->batch > 1 && std::abs(a->y_batch) < a->dim) || (a->length > 1 && std::abs(a->y_token) < a->dim) ||
+        (a->heads > 1 && std::abs(a->y_head) < a->dim))
+        return fail(RPFQ_ERR_INVALID, "%s: heads of y lie over one another: y overlaps itself", who);
     const int64_t run = a->dim * static_cast<int64_t>(esize);
     if (a->x != a->y && share_bytes(a->x, run, a->y, run,
                                     {{a->batch, a->x_batch * esize, a->batch, a->y_batch * esize},

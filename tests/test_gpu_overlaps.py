@@ -92,3 +92,16 @@ def test_codes_beside_their_rows(cuda):
     want = ops.quantize_rows(x)
     assert torch.equal(codes, want[0]) and torch.equal(scale, want[1]) and torch.equal(rows, x)
     assert (buf[:, 3 * k:] == 0).all()
+
+
+def test_rotary_output_over_itself_is_refused(cuda):
+    from rpfq_review_b200 import ops
+    f, pos = ops.rotary_frequencies(16, device=cuda)[0], torch.arange(6, device=cuda)
+    x, flat = torch.randn(6, 2, 16, device=cuda), torch.zeros(400, device=cuda)
+    for strides in ((8, 64, 1), (32, 15, 1), (0, 16, 1)):
+        with pytest.raises(ValueError):
+            ops.rotary(x, pos, f, out=flat.as_strided((6, 2, 16), strides))
+    out = flat.as_strided((6, 2, 16), (16, 96, 1))  # heads outermost
+    assert torch.equal(ops.rotary(x, pos, f, out=out), ops.rotary(x, pos, f))
+    one = flat.as_strided((1, 1, 16), (0, 0, 1))  # strides that no step uses
+    assert torch.equal(ops.rotary(x[:1, :1], pos[:1], f, out=one), ops.rotary(x[:1, :1], pos[:1], f))

@@ -97,3 +97,12 @@ def test_quantize_rows_refuses_outputs_over_what_is_read(f32, bad, word):
     assert L.rpfq_quantize_rows_sm100(a["x"], f32, 8 if f32 else 16, a["q"], 32, a["scale"], 4, 8,
                                       None) == _lib.RPFQ_ERR_INVALID
     assert word in L.rpfq_last_error()
+
+
+@pytest.mark.parametrize("strides", [dict(y_token=0), dict(y_head=0), dict(y_batch=0), dict(y_head=63), dict(y_token=-63),
+                                     dict(y_batch=1)])
+def test_rotary_refuses_an_output_over_itself(strides):
+    rc, message = _rotary(**strides)
+    assert rc == _lib.RPFQ_ERR_INVALID and b"itself" in message, message
+    rc, message = _rotary(y=MB, **dict(strides, **{k.replace("y", "x"): v for k, v in strides.items()}))
+    assert rc == _lib.RPFQ_ERR_INVALID and b"itself" in message, message

@@ -93,8 +93,9 @@ class PackedPhaseLinear(nn.Module):
     (half the memory of the fp16 matrix), every call quantizes its activations
     to 8 bits with a scale per token (``ops.linear_int8``). It takes the place of
     the activation quantizers above and needs ``cache_dense=True``. Planes that
-    are loaded, written, moved or replaced are quantized again by the next call;
-    only a write into planes that were made in inference mode does not show:
+    are loaded, written, moved or replaced are quantized again by the next call.
+    A write that raises no version of a plane (through ``.data``, by a collective
+    or a replayed graph, or into planes made in inference mode) does not show:
     call :meth:`prepack` after it.
     """
 
@@ -234,10 +235,12 @@ class PackedPhaseLinear(nn.Module):
         return dense
 
     def prepack(self) -> torch.Tensor:
-        """Decode the packed planes once (K1). Layers whose real dims are not
+        """Decode the packed planes once (K1), and read the bias again. Layers whose real dims are not
         multiples of 8 keep a zero-padded copy ``[N8, K8]`` for the GEMM. With
         ``compute="int8"`` the decoded rows are quantized and only their codes
         and scales are kept (in the same memory when planes change); returns the codes."""
+        if self._bias32 is not None:
+            self._bias32 = (None, self._bias32[1])
         if self.compute == "int8":
             self._planes8 = None
             return self._int8_weight()[0]
@@ -253,7 +256,8 @@ class PackedPhaseLinear(nn.Module):
         the GEMM epilogue directly). ``residual`` (fp16 or fp32) is added in
         the epilogue and may be ``out`` itself. ``prequantized=True`` skips the
         activation quantization (already applied by the producer, e.g. the
-        fused LayerNorm kernel)."""
+        fused LayerNorm kernel); with ``compute="int8"``, whose rows are quantized
+        by the product's own call, it changes nothing."""
         if out_dtype is None:
             out_dtype = out.dtype if out is not None else (x.dtype if x.dtype in (torch.float16, torch.float32)
                                                            else torch.float16)

@@ -156,3 +156,13 @@ def test_copies_make_their_own_codes(calls):
         got = _run(other)
         assert _same(got, other) and (got[2] == 3).all()
         assert _same(_run(layer), layer) and layer._bias_f32().ne(3).any()
+
+
+def test_prepack_after_writes_that_raise_no_version(calls):
+    layer = _layer(1)
+    _run(layer)
+    layer.u_s0.codes.data.add_(1)
+    layer.bias.data.fill_(5)
+    layer.prepack()
+    got = _run(layer)
+    assert _same(got, layer) and (got[2] == 5).all()

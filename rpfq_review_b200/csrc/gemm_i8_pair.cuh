@@ -17,7 +17,12 @@
 // The accumulator is released as soon as the warp's last part of it is in
 // registers, by an arrival without release semantics: a release waits for the
 // warp's other memory traffic, which the MMA warp does not read (m = 50432, k =
-// 1024, n = 4096: 150 us without GELU against 174..191 with a release).
+// 1024, n = 4096: 150 us without GELU against 174..191 with a release). TMEM is
+// not ordered by releases and acquires but by PTX's rule for tcgen05 operations of
+// different threads: every lane's loads have completed at its tcgen05.wait::ld, its
+// tcgen05.fence::before_thread_sync puts them before what follows in execution
+// (__syncwarp, then lane 0's arrival), and the MMA warp issues behind a
+// tcgen05.fence::after_thread_sync that follows the wait which saw the arrivals.
 //
 // The loops of warps 0 and 1 run on all lanes with only the issuing instruction
 // predicated. On one lane the MMA warp took over 800 cycles for the instructions of

@@ -140,7 +140,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 }
 
 // The same without release semantics, for arrivals that guard no memory of this
-// thread (a TMEM buffer whose loads have completed).
+// thread: a TMEM buffer whose loads have completed (tcgen05.wait::ld), with
+// tcgen05.fence::before_thread_sync before the arrival and ::after_thread_sync behind
+// the wait for it, which order tcgen05 operations without the barrier's help.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

@@ -517,10 +517,9 @@ _ROTARY_MAX_HEADS = 2 ** 24
 _ROTARY_MAX_DIM = 2 ** 31 - 1
 
 
-def _at_most(name: str, what: str, value: int, limit: int) -> None:
+def _too_large(name: str, what: str, value: int, limit: int):
     """What the C structures hold in 32 bits is refused here: there it would come out small."""
-    if value > limit:
-        raise NotImplementedError(f"{name}: {what} must be at most {limit}, got {value}")
+    return NotImplementedError(f"{name}: {what} must be at most {limit}, got {value}")
 
 
 def _tensors(name: str, index: int, tensors) -> None:
@@ -597,7 +596,8 @@ def quantize_rows(x: torch.Tensor):
     if not shape or shape[-1] == 0:
         raise ValueError(f"quantize_rows: x must be [..., k] with k > 0, got {tuple(shape)}")
     k, lead = shape[-1], shape[:-1]
-    _at_most("quantize_rows", "k", k, _QUANTIZE_MAX_K)
+    if k > _QUANTIZE_MAX_K:
+        raise _too_large("quantize_rows", "k", k, _QUANTIZE_MAX_K)
     x2, m, ldx = _matrix(x, k, "x")
     ld = (k + 15) // 16 * 16
     q = x.new_empty((*lead, ld), dtype=torch.int8)
@@ -684,8 +684,10 @@ def _check_codes(name: str, w: torch.Tensor) -> None:
     if w.dtype is not torch.int8 or w.dim() != 2 or w.numel() == 0:
         raise ValueError(f"{name}: w must be int8 [n, k] with n, k > 0, got {w.dtype} {tuple(w.shape)}")
     n, k = w.shape
-    _at_most(name, "k", k, GEMM_INT8_MAX_K)
-    _at_most(name, "n", n, _GEMM_INT8_MAX_N)
+    if k > GEMM_INT8_MAX_K:
+        raise _too_large(name, "k", k, GEMM_INT8_MAX_K)
+    if n > _GEMM_INT8_MAX_N:
+        raise _too_large(name, "n", n, _GEMM_INT8_MAX_N)
 
 
 def gemm_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -818,8 +820,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     if inv_freq.dtype is not torch.float64:
         raise ValueError(f"{name}: inv_freq must be float64, got {inv_freq.dtype}")
     B, L, H, D = x.shape if four else (1, *x.shape)
-    _at_most(name, "heads", H, _ROTARY_MAX_HEADS)
-    _at_most(name, "the head dim", D, _ROTARY_MAX_DIM)
+    if H > _ROTARY_MAX_HEADS:
+        raise _too_large(name, "heads", H, _ROTARY_MAX_HEADS)
+    if D > _ROTARY_MAX_DIM:
+        raise _too_large(name, "the head dim", D, _ROTARY_MAX_DIM)
     pairs = inv_freq.numel()
     if pairs == 0 or 2 * pairs > D or pairs % axes:
         raise ValueError(f"{name}: inv_freq must hold 1..{D // 2} values, a multiple of axes, got {pairs}")

@@ -957,10 +957,15 @@ bool i8_vec_out(const RpfqGemmI8Args* a) {
 }
 
 // Rows that the few-row kernel takes; their codes lie in its shared memory. Up to
-// four it is ahead of the tensor-core tiles (us, few / tiles at n x k: 1 row 1024 x
-// 4096 2.3 / 4.6; 4 rows 768 x 768 2.3 / 3.1, 4096 x 4096 6.0 / 5.7); with rows to
-// quantize the tiles need a launch more, which up to eight rows of at most 2048
-// values repays (8 rows 768 x 768 3.6 / 5.3, 1024 x 4096 10.5 / 7.1).
+// four, where w is a few MB, it is ahead of the tensor-core tiles (us, few / tiles at
+// n x k, w from DRAM: 1 row 1024 x 4096 2.7 / 4.7, 4096 x 4096 4.5 / 6.7; 4 rows 768 x
+// 768 2.2 / 2.7, 1024 x 4096 4.6 / 4.8); with rows to quantize the tiles need a launch
+// more, which up to eight rows of at most 2048 values repays (8 rows 768 x 768 3.5 /
+// 4.5, 4096 x 1024 3.8 / 5.7; 1024 x 4096 10.5 / 7.1). It bounds neither n nor, up to
+// four rows, k: about even at 16 MB of w (4 rows 4096 x 4096 6.9 / 6.7, quantized 9.0 /
+// 8.4), and behind beyond it from two rows on (4096 x 16384: 1 row 13.5 / 14.8,
+// quantized 18.9 / 16.9, 2 rows 15.8 / 14.7, 4 rows 25 / 15, quantized 36 / 17) and for
+// long rows (4 rows 1000 x 24576 20 / 11, quantized 35 / 15).
 bool few_rows_fit(int64_t m, int64_t k, bool quantize) {
     return (m <= 4 || (quantize && m <= kFewRows && k <= 2048)) && m * ((k + 15) / 16 * 16) <= kFewSmem;
 }

@@ -179,7 +179,7 @@ class PackedPhaseLinear(nn.Module):
         bias tensor changes."""
         if self._bias32 is not None and _unchanged(self._bias32[0], (self.bias,)):
             return self._bias32[1]
-        bias = self.bias.float()
+        bias = self.bias.to(torch.float32, copy=True)
         if not _capturing(self.bias) and not self.bias.is_inference():
             record = _made_from((self.bias,))
             (bias,) = _keep(None if self._bias32 is None else self._bias32[1:], (bias,))

@@ -166,3 +166,17 @@ def test_prepack_after_writes_that_raise_no_version(calls):
     layer.prepack()
     got = _run(layer)
     assert _same(got, layer) and (got[2] == 5).all()
+
+
+def test_fp32_bias_stays_the_callers(calls):
+    """A bias that is fp32 already is copied, not kept itself and written over later."""
+    layer = _layer(1)
+    first = torch.full((16,), 2.0)
+    layer.bias = first
+    assert (_run(layer)[2] == 2).all()
+    layer.bias = torch.full((16,), 3.0)
+    assert (_run(layer)[2] == 3).all() and (first == 2).all()
+    layer.bias.fill_(4)
+    assert (_run(layer)[2] == 4).all()
+    version, kept = layer.bias._version, layer._bias32
+    assert (_run(layer)[2] == 4).all() and layer.bias._version == version and layer._bias32 is kept

@@ -192,12 +192,25 @@ class PackedPhaseLinear(nn.Module):
         planes = self._plane_tensors()
         if _unchanged(self._planes8, planes):
             return self.codes8, self.scale8
+        self._check_planes()
         record = _made_from(planes)
         codes, scale = ops.quantize_rows(ops.prepack(self.packed(), self.rounding))
         if not _capturing(codes):
             codes, scale = _keep(None if self.codes8 is None else (self.codes8, self.scale8), (codes, scale))
             self.codes8, self.scale8, self._planes8 = codes, scale, record
         return codes, scale
+
+    def _check_planes(self) -> None:
+        """The decoder reads contiguous uint8 codes and fp16 gammas of one device; after a cast, a
+        move or an assignment they may be something else."""
+        codes = self.u_s0.codes
+        gammas = (codes.shape[0], codes.shape[1] * 8 // self.code_bits // BLOCK_SIZE)
+        for name, plane in self.named_children():
+            for what, t in plane._buffers.items():
+                dtype, shape = (torch.uint8, tuple(codes.shape)) if what == "codes" else (torch.float16, gammas)
+                if t.dtype != dtype or t.shape != shape or t.device != codes.device or not t.is_contiguous():
+                    raise ValueError(f"{name}.{what} must be a contiguous {dtype} {shape} on {codes.device}, got {t.dtype} "
+                                     f"{tuple(t.shape)} on {t.device}")
 
     def _plane_tensors(self):
         return [t for tag in ("u", "w") for s in range(self.stages)

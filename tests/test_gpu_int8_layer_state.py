@@ -126,3 +126,28 @@ def test_layer_made_in_inference_mode(cuda):
         other = _layer(3)
         other.u_s0.codes.fill_(0)
         assert torch.equal(layer(x), other(x))
+
+
+def test_planes_of_other_types_places_and_shapes_are_refused(cuda):
+    """A cast module, a plane left on the CPU, one of another size or order: the decoder would
+    read their bytes as something else."""
+    from rpfq_review_b200 import PackedPhaseLinear
+    from rpfq_review_b200.packing import random_packed
+    x = _x()
+    layer = lambda: PackedPhaseLinear.from_packed(random_packed(96, 64, seed=1, device=cuda), compute="int8")  # noqa: E731
+    want = layer()(x)
+    for cast in (torch.float32, torch.bfloat16):
+        other = layer()
+        other.to(cast)
+        with pytest.raises(ValueError, match="float16"):
+            other(x)
+        other.to(torch.float16)
+        assert cast == torch.bfloat16 or torch.equal(other(x), want)
+    for name, value in (("gamma_real", lambda t: t.cpu()), ("codes", lambda t: t.cpu()), ("codes", lambda t: t[:-1]),
+                        ("gamma_imag", lambda t: t[:-1]), ("codes", lambda t: t.t().contiguous().t()),
+                        ("codes", lambda t: t.view(torch.int8))):
+        other = layer()
+        plane = other.w_s1
+        plane._buffers[name] = value(plane._buffers[name])
+        with pytest.raises(ValueError, match=f"w_s1.{name}"):
+            other(x)

@@ -168,8 +168,8 @@ int rpfq_act_quant_sm100(const uint16_t* x, int64_t ldx, uint16_t* xq, int64_t l
  * (fp32 with x_f32 != 0), row stride ldx; q is [m, k] int8, row stride ldq.
  *   t = max(amax |x|, 1e-30); q = rint(fl(x * fl(fl(1 / t) * 127))); scale = t / 127
  * (half to even, fp32 steps). A row with a NaN or an infinity gets codes of
- * zero and a scale of NaN. q, scale and x share no memory. No counterpart in the reference, whose quantizers
- * return to fp16 (ActivationQuantSTE.forward,
+ * zero and a scale of NaN. x, q and scale share no memory. No counterpart in
+ * the reference, whose quantizers return to fp16 (ActivationQuantSTE.forward,
  * RPFQ-ViT-main/quant_models/quant_i.py:442-455). */
 int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                              int64_t m, int32_t k, rpfq_stream_t stream);
@@ -178,11 +178,11 @@ int rpfq_quantize_rows_sm100(const void* x, int32_t x_f32, int64_t ldx, int8_t* 
  * residual[m, n] of int8 codes x [m, k] and w [n, k] with one scale per token
  * and one per output channel: exact int32 sums on the tensor cores, scaled in
  * fp32, fp16 or fp32 output. The 8-bit form of rpfq_gemm_sm100; y may be the
- * residual (the same address and row stride), and shares no other memory with what the call
- * reads or with scratch. Requirements: x and w 16-byte aligned with row strides that are
- * multiples of 16 (any k up to 131071 within such rows); y, residual, bias and
- * the scales aligned to their values, any n and any row strides >= n; the
- * residual has y's dtype. Nothing is kept between calls.
+ * residual (the same address and row stride) and shares no other memory with
+ * scratch or with what the call reads. Requirements: x and w 16-byte aligned with
+ * row strides that are multiples of 16 (any k up to 131071 within such rows); y,
+ * residual, bias and the scales aligned to their values, any n and any row
+ * strides >= n; the residual has y's dtype. Nothing is kept between calls.
  * With RPFQ_GEMM_X_F16 or RPFQ_GEMM_X_F32 in flags, x holds fp16 or fp32
  * activations (any row stride >= k, x_scale unused): their rows are quantized
  * as by rpfq_quantize_rows_sm100, inside the product's launch for a few rows
@@ -231,8 +231,8 @@ enum { RPFQ_POS_I32 = 0, RPFQ_POS_I64 = 1, RPFQ_POS_F32 = 2, RPFQ_POS_F64 = 3 };
  * positions[.., 1]. Angles are formed and reduced in fp64. x and y are fp16
  * (fp32 with f32 != 0) [batch, length, heads, dim] with strides in elements
  * and unit stride inside a head; y may be x (same strides), which leaves the
- * values past 2 * pairs untouched, and shares memory with nothing that is read in any
- * other way. */
+ * values past 2 * pairs untouched. Otherwise y shares no memory with what is
+ * read, and in no case do heads of y lie over one another. */
 typedef struct RpfqRotaryArgs {
     const void* x;
     int64_t x_batch, x_token, x_head;   /* strides                                        */
